@@ -164,6 +164,91 @@ EXTERN_C void launch_dilate_reverse_r64(
   StreamContext stream
 );
 
+/* dst[i,j] = scale * table[tokens[i], j] for m tokens and a table of v rows of n elements. tokens are */
+/* signed integers on the device, id_bytes (4 or 8) wide each; an id outside [0, v) (a padded place) */
+/* gives a row of zeros. No reference kernel exists; the nearest is the row broadcast */
+/* (src/cuda/nvcc_src/broadcast_j_ij.cu:9-57). dst must not overlap the table. */
+EXTERN_C void launch_embedding_i_ij_r16(
+  const void* table,
+  const void* tokens,
+  void* dst,
+  double scale,
+  len_t id_bytes,
+  len_t v,
+  len_t m,
+  len_t n,
+  StreamContext stream
+);
+EXTERN_C void launch_embedding_i_ij_r32(
+  const void* table,
+  const void* tokens,
+  void* dst,
+  double scale,
+  len_t id_bytes,
+  len_t v,
+  len_t m,
+  len_t n,
+  StreamContext stream
+);
+EXTERN_C void launch_embedding_i_ij_r64(
+  const void* table,
+  const void* tokens,
+  void* dst,
+  double scale,
+  len_t id_bytes,
+  len_t v,
+  len_t m,
+  len_t n,
+  StreamContext stream
+);
+
+/* table_grads[k,j] = scale * sum of dst_grads[i,j] over the places i with tokens[i] == k */
+/*                    + alpha*table_grads[k,j] */
+/* for every row k of the table, the ones no token names among them (alpha = 0 clears those and never */
+/* reads table_grads; alpha = 1 leaves them untouched). tokens and id_bytes as in embedding_i_ij; the */
+/* gradient of a padded place is not read into any sum. scratch is caller-owned workspace of */
+/* mpEmbeddingReverseScratchBytes(dtype, v, m, n) bytes, 16-byte aligned; launches that may overlap in */
+/* time get different workspaces. Results do not change from run to run. */
+EXTERN_C void launch_embedding_i_ij_reverse_r16(
+  const void* tokens,
+  const void* dst_grads,
+  void* table_grads,
+  void* scratch,
+  double scale,
+  double alpha,
+  len_t id_bytes,
+  len_t v,
+  len_t m,
+  len_t n,
+  StreamContext stream
+);
+EXTERN_C void launch_embedding_i_ij_reverse_r32(
+  const void* tokens,
+  const void* dst_grads,
+  void* table_grads,
+  void* scratch,
+  double scale,
+  double alpha,
+  len_t id_bytes,
+  len_t v,
+  len_t m,
+  len_t n,
+  StreamContext stream
+);
+EXTERN_C void launch_embedding_i_ij_reverse_r64(
+  const void* tokens,
+  const void* dst_grads,
+  void* table_grads,
+  void* scratch,
+  double scale,
+  double alpha,
+  len_t id_bytes,
+  len_t v,
+  len_t m,
+  len_t n,
+  StreamContext stream
+);
+
 /* dev_a = value. Replaces src/cuda/nvcc_src/fill.cu:4-27; seeds dL/dz = 1 on the reverse path */
 /* (src/core/graph.zig:116). */
 EXTERN_C void launch_fill_r16(
@@ -623,6 +708,106 @@ EXTERN_C void launch_fused_selu_hadamard_sub_reverse_r64(
   StreamContext stream
 );
 
+/* gradient_norm (alpha = 0) and gradient_scale of the same `count` tensors in one call: norm[0] gets */
+/* their norm, clipped_k = grads_k * min(1, max_norm / norm[0]). Arguments and workspace as there. */
+EXTERN_C void launch_gradient_clip_r16(
+  const void* grads,
+  const void* clipped,
+  const void* sizes,
+  void* norm,
+  void* scratch,
+  double max_norm,
+  len_t count,
+  StreamContext stream
+);
+EXTERN_C void launch_gradient_clip_r32(
+  const void* grads,
+  const void* clipped,
+  const void* sizes,
+  void* norm,
+  void* scratch,
+  double max_norm,
+  len_t count,
+  StreamContext stream
+);
+EXTERN_C void launch_gradient_clip_r64(
+  const void* grads,
+  const void* clipped,
+  const void* sizes,
+  void* norm,
+  void* scratch,
+  double max_norm,
+  len_t count,
+  StreamContext stream
+);
+
+/* norm[0] = sqrt(sum of g^2 over every element of `count` tensors + alpha * norm[0]^2). grads and sizes */
+/* are host arrays of `count` device addresses and of `count` element counts (len_t), read before the */
+/* call returns; norm is one double on the device. alpha = 0 never reads norm, alpha = 1 adds tensors of */
+/* another type or place to what an earlier call found. Sums run in fp64 in a fixed order. scratch is */
+/* caller-owned workspace of mpGradientNormScratchBytes(dtype, count) bytes, 8-byte aligned. No reference */
+/* kernel exists. */
+EXTERN_C void launch_gradient_norm_r16(
+  const void* grads,
+  const void* sizes,
+  void* norm,
+  void* scratch,
+  double alpha,
+  len_t count,
+  StreamContext stream
+);
+EXTERN_C void launch_gradient_norm_r32(
+  const void* grads,
+  const void* sizes,
+  void* norm,
+  void* scratch,
+  double alpha,
+  len_t count,
+  StreamContext stream
+);
+EXTERN_C void launch_gradient_norm_r64(
+  const void* grads,
+  const void* sizes,
+  void* norm,
+  void* scratch,
+  double alpha,
+  len_t count,
+  StreamContext stream
+);
+
+/* clipped_k = grads_k * min(1, max_norm / norm[0]) for `count` tensors, with the norm that an earlier */
+/* gradient_norm left on the device (tensors of several types: one gradient_norm each, alpha = 1 from the */
+/* second on, then one gradient_scale each). grads, clipped and sizes are host arrays as in */
+/* gradient_norm; clipped_k may be grads_k, and a norm of at most max_norm then writes nothing. A norm */
+/* that is infinite or NaN gives zeros and NaNs as the formula does: the caller sees it in norm. */
+EXTERN_C void launch_gradient_scale_r16(
+  const void* grads,
+  const void* clipped,
+  const void* sizes,
+  const void* norm,
+  double max_norm,
+  len_t count,
+  StreamContext stream
+);
+EXTERN_C void launch_gradient_scale_r32(
+  const void* grads,
+  const void* clipped,
+  const void* sizes,
+  const void* norm,
+  double max_norm,
+  len_t count,
+  StreamContext stream
+);
+EXTERN_C void launch_gradient_scale_r64(
+  const void* grads,
+  const void* clipped,
+  const void* sizes,
+  const void* norm,
+  double max_norm,
+  len_t count,
+  StreamContext stream
+);
+
 /* c = a * b. Replaces src/cuda/nvcc_src/hadamard.cu:3-29. */
 EXTERN_C void launch_hadamard_r16(
   const void* a,
@@ -760,6 +945,93 @@ EXTERN_C void launch_inner_product_ji_jk_ik_r64(
   void* c_data,
   double beta,
   len_t m, len_t n, len_t k,
+  StreamContext stream
+);
+
+/* dst[i,j] = (src[i,j] - mean_j src[i,:]) / sqrt(var_j src[i,:] + eps) * gain[j] + bias[j], with the */
+/* variance over n (not n - 1). gain NULL counts as ones, bias NULL as zeros. No reference kernel */
+/* exists; scalars cross the boundary as double and sizes as len_t like every reference launcher */
+/* (src/cuda/nvcc_src/reduce_ij_i.cu:35-42). dst may be src. */
+EXTERN_C void launch_layernorm_ij_j_r16(
+  const void* src,
+  const void* gain,
+  const void* bias,
+  void* dst,
+  double eps,
+  len_t m,
+  len_t n,
+  StreamContext stream
+);
+EXTERN_C void launch_layernorm_ij_j_r32(
+  const void* src,
+  const void* gain,
+  const void* bias,
+  void* dst,
+  double eps,
+  len_t m,
+  len_t n,
+  StreamContext stream
+);
+EXTERN_C void launch_layernorm_ij_j_r64(
+  const void* src,
+  const void* gain,
+  const void* bias,
+  void* dst,
+  double eps,
+  len_t m,
+  len_t n,
+  StreamContext stream
+);
+
+/* With u_i and r_i = 1/sqrt(variance + eps) of row i of src, h = (src - u_i) * r_i and */
+/* e = dst_grads * gain (gain NULL: ones): */
+/*   src_grads[i,j] = r_i * (e[i,j] - mean_j e[i,:] - h[i,j] * mean_j(e*h)[i,:]) + alpha*src_grads[i,j] */
+/*   gain_grads[j]  = sum_i dst_grads[i,j] * h[i,j]                              + alpha*gain_grads[j] */
+/*   bias_grads[j]  = sum_i dst_grads[i,j]                                       + alpha*bias_grads[j] */
+/* gain_grads or bias_grads that is NULL is not computed; src_grads may be dst_grads or src. alpha = 0 */
+/* never reads the three results. scratch is caller-owned workspace of */
+/* mpLayernormReverseScratchBytes(dtype, m, n) bytes (the reference hands kernels their workspace from */
+/* the per-stream scratch, src/core/utils.zig:20-36). Results do not change from run to run. */
+EXTERN_C void launch_layernorm_ij_j_reverse_r16(
+  const void* src,
+  const void* gain,
+  const void* dst_grads,
+  void* src_grads,
+  void* gain_grads,
+  void* bias_grads,
+  void* scratch,
+  double eps,
+  double alpha,
+  len_t m,
+  len_t n,
+  StreamContext stream
+);
+EXTERN_C void launch_layernorm_ij_j_reverse_r32(
+  const void* src,
+  const void* gain,
+  const void* dst_grads,
+  void* src_grads,
+  void* gain_grads,
+  void* bias_grads,
+  void* scratch,
+  double eps,
+  double alpha,
+  len_t m,
+  len_t n,
+  StreamContext stream
+);
+EXTERN_C void launch_layernorm_ij_j_reverse_r64(
+  const void* src,
+  const void* gain,
+  const void* dst_grads,
+  void* src_grads,
+  void* gain_grads,
+  void* bias_grads,
+  void* scratch,
+  double eps,
+  double alpha,
+  len_t m,
+  len_t n,
   StreamContext stream
 );
 
@@ -1258,6 +1530,9 @@ EXTERN_C len_t mpSoftmaxScratchBytes(len_t dtype, len_t m, len_t n);
 EXTERN_C len_t mpSoftmaxReverseScratchBytes(len_t dtype, len_t m, len_t n);
 EXTERN_C len_t mpReduceScratchBytes(len_t dtype, len_t m, len_t n);
 EXTERN_C len_t mpRmsnormScratchBytes(len_t dtype, len_t m, len_t n);
+EXTERN_C len_t mpLayernormReverseScratchBytes(len_t dtype, len_t m, len_t n);
+EXTERN_C len_t mpEmbeddingReverseScratchBytes(len_t dtype, len_t v, len_t m, len_t n);
+EXTERN_C len_t mpGradientNormScratchBytes(len_t dtype, len_t count);
 /* launch_rmsnorm_ij_j_reverse_r32 without the scratch argument, for callers that cannot allocate a
  * workspace (code under HIP graph capture, serving loops, harnesses that forbid hipMalloc): the partial
  * gain rows go into a 16 MiB device array that the library holds on every GPU it runs on. It has no

@@ -2,6 +2,9 @@
  * Exports of the kernel library that are not per-dtype launchers: workspace sizing and (test
  * build only) the row-regime and cluster-tuning overrides. Compiled once (no `Scalar` replication).
  */
+#include "embedding.h"
+#include "gradient_norm.h"
+#include "row_layernorm.h"
 #include "row_reduce.h"
 #include "row_softmax.h"
 
@@ -59,6 +62,37 @@ extern "C" len_t mpReduceScratchBytes(len_t dtype, len_t m, len_t n) {
     case MP_R64: return mp::reduce_cols_scratch_bytes<r64>(m, n);
     default: mp::require(false, "mpReduceScratchBytes: dtype must be 0, 1 or 2"); return 0;
   }
+}
+
+// Bytes of caller-owned scratch that launch_layernorm_ij_j_reverse_<dtype> needs for an [m, n] problem:
+// two rows of n accumulators (for the gain and the bias) per workgroup, at most two workgroups per
+// compute unit.
+extern "C" len_t mpLayernormReverseScratchBytes(len_t dtype, len_t m, len_t n) {
+  switch (dtype) {
+    case MP_R16: return mp::layernorm_reverse_scratch_bytes<r16>(m, n);
+    case MP_R32: return mp::layernorm_reverse_scratch_bytes<r32>(m, n);
+    case MP_R64: return mp::layernorm_reverse_scratch_bytes<r64>(m, n);
+    default: mp::require(false, "mpLayernormReverseScratchBytes: dtype must be 0, 1 or 2"); return 0;
+  }
+}
+
+// Bytes of caller-owned scratch that launch_embedding_i_ij_reverse_<dtype> needs for m tokens and a
+// table of v rows of n: the sorted places, and two rows of n accumulators per chunk of them.
+extern "C" len_t mpEmbeddingReverseScratchBytes(len_t dtype, len_t v, len_t m, len_t n) {
+  mp::require(v < 0xffffffffull, "mpEmbeddingReverseScratchBytes: the table must have fewer than 2^32 - 1 rows");
+  switch (dtype) {
+    case MP_R16: return mp::embedding_scratch<r16>(m, n).bytes;
+    case MP_R32: return mp::embedding_scratch<r32>(m, n).bytes;
+    case MP_R64: return mp::embedding_scratch<r64>(m, n).bytes;
+    default: mp::require(false, "mpEmbeddingReverseScratchBytes: dtype must be 0, 1 or 2"); return 0;
+  }
+}
+
+// Bytes of caller-owned scratch that launch_gradient_norm_<dtype> and launch_gradient_clip_<dtype> need
+// for `count` tensors: the partial sums, in fp64 for every dtype.
+extern "C" len_t mpGradientNormScratchBytes(len_t dtype, len_t count) {
+  mp::require(dtype <= MP_R64, "mpGradientNormScratchBytes: dtype must be 0, 1 or 2");
+  return mp::gradient_norm_scratch_bytes(count);
 }
 
 #ifdef MP_DIAGNOSTICS

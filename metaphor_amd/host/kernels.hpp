@@ -27,6 +27,8 @@ inline const DispatchArray<decltype(launch_broadcast_j_ij_r16)> broadcast_j_ij{{
 inline const DispatchArray<decltype(launch_copy_r16)> copy{{launch_copy_r16, launch_copy_r32, launch_copy_r64}};
 inline const DispatchArray<decltype(launch_dilate_r16)> dilate{{launch_dilate_r16, launch_dilate_r32, launch_dilate_r64}};
 inline const DispatchArray<decltype(launch_dilate_reverse_r16)> dilate_reverse{{launch_dilate_reverse_r16, launch_dilate_reverse_r32, launch_dilate_reverse_r64}};
+inline const DispatchArray<decltype(launch_embedding_i_ij_r16)> embedding_i_ij{{launch_embedding_i_ij_r16, launch_embedding_i_ij_r32, launch_embedding_i_ij_r64}};
+inline const DispatchArray<decltype(launch_embedding_i_ij_reverse_r16)> embedding_i_ij_reverse{{launch_embedding_i_ij_reverse_r16, launch_embedding_i_ij_reverse_r32, launch_embedding_i_ij_reverse_r64}};
 inline const DispatchArray<decltype(launch_fill_r16)> fill{{launch_fill_r16, launch_fill_r32, launch_fill_r64}};
 inline const DispatchArray<decltype(launch_fused_add_add_r16)> fused_add_add{{launch_fused_add_add_r16, launch_fused_add_add_r32, launch_fused_add_add_r64}};
 inline const DispatchArray<decltype(launch_fused_add_add_reverse_r16)> fused_add_add_reverse{{launch_fused_add_add_reverse_r16, launch_fused_add_add_reverse_r32, launch_fused_add_add_reverse_r64}};
@@ -40,11 +42,16 @@ inline const DispatchArray<decltype(launch_fused_selu_hadamard_add_add_r16)> fus
 inline const DispatchArray<decltype(launch_fused_selu_hadamard_add_add_reverse_r16)> fused_selu_hadamard_add_add_reverse{{launch_fused_selu_hadamard_add_add_reverse_r16, launch_fused_selu_hadamard_add_add_reverse_r32, launch_fused_selu_hadamard_add_add_reverse_r64}};
 inline const DispatchArray<decltype(launch_fused_selu_hadamard_sub_r16)> fused_selu_hadamard_sub{{launch_fused_selu_hadamard_sub_r16, launch_fused_selu_hadamard_sub_r32, launch_fused_selu_hadamard_sub_r64}};
 inline const DispatchArray<decltype(launch_fused_selu_hadamard_sub_reverse_r16)> fused_selu_hadamard_sub_reverse{{launch_fused_selu_hadamard_sub_reverse_r16, launch_fused_selu_hadamard_sub_reverse_r32, launch_fused_selu_hadamard_sub_reverse_r64}};
+inline const DispatchArray<decltype(launch_gradient_clip_r16)> gradient_clip{{launch_gradient_clip_r16, launch_gradient_clip_r32, launch_gradient_clip_r64}};
+inline const DispatchArray<decltype(launch_gradient_norm_r16)> gradient_norm{{launch_gradient_norm_r16, launch_gradient_norm_r32, launch_gradient_norm_r64}};
+inline const DispatchArray<decltype(launch_gradient_scale_r16)> gradient_scale{{launch_gradient_scale_r16, launch_gradient_scale_r32, launch_gradient_scale_r64}};
 inline const DispatchArray<decltype(launch_hadamard_r16)> hadamard{{launch_hadamard_r16, launch_hadamard_r32, launch_hadamard_r64}};
 inline const DispatchArray<decltype(launch_hadamard_reverse_r16)> hadamard_reverse{{launch_hadamard_reverse_r16, launch_hadamard_reverse_r32, launch_hadamard_reverse_r64}};
 inline const DispatchArray<decltype(launch_inner_product_ij_jk_ik_r16)> inner_product_ij_jk_ik{{launch_inner_product_ij_jk_ik_r16, launch_inner_product_ij_jk_ik_r32, launch_inner_product_ij_jk_ik_r64}};
 inline const DispatchArray<decltype(launch_inner_product_ij_kj_ik_r16)> inner_product_ij_kj_ik{{launch_inner_product_ij_kj_ik_r16, launch_inner_product_ij_kj_ik_r32, launch_inner_product_ij_kj_ik_r64}};
 inline const DispatchArray<decltype(launch_inner_product_ji_jk_ik_r16)> inner_product_ji_jk_ik{{launch_inner_product_ji_jk_ik_r16, launch_inner_product_ji_jk_ik_r32, launch_inner_product_ji_jk_ik_r64}};
+inline const DispatchArray<decltype(launch_layernorm_ij_j_r16)> layernorm_ij_j{{launch_layernorm_ij_j_r16, launch_layernorm_ij_j_r32, launch_layernorm_ij_j_r64}};
+inline const DispatchArray<decltype(launch_layernorm_ij_j_reverse_r16)> layernorm_ij_j_reverse{{launch_layernorm_ij_j_reverse_r16, launch_layernorm_ij_j_reverse_r32, launch_layernorm_ij_j_reverse_r64}};
 inline const DispatchArray<decltype(launch_negate_r16)> negate{{launch_negate_r16, launch_negate_r32, launch_negate_r64}};
 inline const DispatchArray<decltype(launch_permutate_ij_ji_r16)> permutate_ij_ji{{launch_permutate_ij_ji_r16, launch_permutate_ij_ji_r32, launch_permutate_ij_ji_r64}};
 inline const DispatchArray<decltype(launch_reduce_ij_i_r16)> reduce_ij_i{{launch_reduce_ij_i_r16, launch_reduce_ij_i_r32, launch_reduce_ij_i_r64}};

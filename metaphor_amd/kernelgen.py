@@ -168,6 +168,9 @@ def make_kernel_declarations():
         "EXTERN_C len_t mpSoftmaxReverseScratchBytes(len_t dtype, len_t m, len_t n);",
         "EXTERN_C len_t mpReduceScratchBytes(len_t dtype, len_t m, len_t n);",
         "EXTERN_C len_t mpRmsnormScratchBytes(len_t dtype, len_t m, len_t n);",
+        "EXTERN_C len_t mpLayernormReverseScratchBytes(len_t dtype, len_t m, len_t n);",
+        "EXTERN_C len_t mpEmbeddingReverseScratchBytes(len_t dtype, len_t v, len_t m, len_t n);",
+        "EXTERN_C len_t mpGradientNormScratchBytes(len_t dtype, len_t count);",
         "/* launch_rmsnorm_ij_j_reverse_r32 without the scratch argument, for callers that cannot allocate a",
         " * workspace (code under HIP graph capture, serving loops, harnesses that forbid hipMalloc): the partial",
         " * gain rows go into a 16 MiB device array that the library holds on every GPU it runs on. It has no",
