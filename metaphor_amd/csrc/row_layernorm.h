@@ -163,27 +163,64 @@ __global__ __launch_bounds__(STREAM_THREADS) void layernorm_rev_stream(
  * a row is held by SUB lanes, 64 / SUB rows a wavefront; SUB = 64: by `gw` wavefronts, any number up
  * to 16 (a kernel argument), so that rows of any length leave fewer than 64 lanes' worth of packs idle.
  * Loads have no conditions: a pack beyond the row reads its first pack and is left out of every
- * sum. */
+ * sum. The pack that the row's end cuts (LOOSE) is read whole too, into the next row, and masked by the
+ * one lane that holds it; only where that would pass the tensor's end are its elements read singly. */
 template <class T, int W, int SUB, int NV, bool LOOSE> struct NormRow {
   using P = typename precision<T>::type;
   using V = typename vec_of<T, W>::type;
+  using VL = typename std::conditional<LOOSE, typename loose_vec_of<T, W>::type, V>::type;
   const RowPacks<T, W, LOOSE> rp;
   int lanes, lane; /* lanes a row, and which of them this is */
 
   __device__ __forceinline__ NormRow(size_t n, int lanes_, int lane_) : rp(n), lanes(lanes_), lane(lane_) {}
   __device__ __forceinline__ int pack(int k) const { return k * lanes + lane; }
   __device__ __forceinline__ bool inside(int k) const { return pack(k) < rp.npk; }
-  template <bool NT> __device__ __forceinline__ void fetch(const T* row, V (&out)[NV]) const {
+  __device__ __forceinline__ bool cut(int k) const { return LOOSE && rp.last != W && pack(k) == rp.npk - 1; }
+  /* whether the packs of this row reach past m rows of n (short rows: not the last one alone) */
+  __device__ __forceinline__ bool ends(size_t row, size_t m, size_t n) const { return row * n + (size_t)rp.npk * W > m * n; }
+  /* a row of x or dy; KEEP: through loads that leave it in the memory-side cache (keep_input, row_cluster.h) */
+  template <bool KEEP> __device__ __forceinline__ void fetch(const T* row, V (&out)[NV], bool end) const {
+    if (LOOSE && end) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) out[k] = rp.template raw<NT>(row, inside(k) ? pack(k) : 0);
+      for (int k = 0; k < NV; ++k) out[k] = rp.template raw<!KEEP>(row, inside(k) ? pack(k) : 0);
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const VL* at = reinterpret_cast<const VL*>(row + (size_t)(unsigned)(inside(k) ? pack(k) : 0) * W);
+      out[k] = KEEP ? *at : __builtin_nontemporal_load(at);
+    }
   }
-  /* elements the wavefront `w` of the row holds (SUB < 64: the row's own) */
-  __device__ __forceinline__ int held(int w, size_t n) const {
+  /* a vector that every row uses; NULL: `fill` throughout */
+  __device__ __forceinline__ void fetch_vector(const T* vec, V (&out)[NV], T fill) const {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      if (vec) {
+        out[k] = rp.template raw<false>(vec, inside(k) ? pack(k) : 0);
+      } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) out[k][i] = fill;
+      }
+    }
+  }
+  /* what a cut pack read behind the row becomes zero */
+  __device__ __forceinline__ void mask(V (&v)[NV]) const {
+    if constexpr (LOOSE)
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+        if (cut(k))
+#pragma unroll
+          for (int i = 0; i < W; ++i) v[k][i] = i < rp.last ? v[k][i] : (T)0;
+  }
+  /* elements the wavefront `w` of the row holds in the first `packs` packs of its lanes (SUB < 64: the
+   * whole row, whose lanes hold one pack each) */
+  __device__ __forceinline__ int held(int w, int depth, size_t n) const {
     if (SUB < WAVE) return (int)n;
     int packs = 0;
     bool end = false;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
+      if (k >= depth) break;
       const int lo = k * lanes + w * WAVE, left = rp.npk - lo;
       packs += left < 0 ? 0 : left > WAVE ? WAVE : left;
       end = end || (left > 0 && left <= WAVE);
@@ -192,79 +229,42 @@ template <class T, int W, int SUB, int NV, bool LOOSE> struct NormRow {
   }
 };
 
-/* What the wavefronts of a row hand each other: a pivot near the mean of a wavefront's own elements, the
- * sums of x - pivot and its square, and in the reverse those of e = dy * gain and e * (x - pivot). Every
- * wavefront takes its sums about a pivot of its own, so one exchange does for the mean and the
- * variance, without a difference of squares of values far from zero. */
-template <class P> struct NormPart { P pivot, off, square, e, ex; };
-template <class P> struct NormStats {
-  P pivot, off, r; /* mean = pivot + off: x - mean is (x - pivot) - off, where x - pivot is exact or nearly so */
-  P mean_e, mean_eh;
-};
-
-/* The row's statistics from the parts of its wavefronts, which lie in LDS behind a barrier; lane i of every
- * 16 takes part i, `held` of whose elements exist (0 from the gw-th on), and all lanes get the same bits. */
-template <bool REVERSE, class P>
-__device__ __forceinline__ NormStats<P> norm_join(const NormPart<P>* parts, int gw, P held, P inv_n, P eps) {
-  const int slot = threadIdx.x & 15;
-  NormPart<P> part = parts[slot < gw ? slot : 0];
-  NormStats<P> s;
-  s.pivot = parts[0].pivot;
-  const bool real = slot < gw;
-  const P apart = part.pivot - s.pivot;
-  s.off = fold_partials<AddOP, 16>(real ? part.off + held * apart : (P)0) * inv_n;
-  const P by = apart - s.off; /* pivot - mean */
-  const P square = fold_partials<AddOP, 16>(real ? part.square + by * ((P)2 * part.off + held * by) : (P)0) * inv_n;
-  s.r = rsqrt_of((square < (P)0 ? (P)0 : square) + eps);
-  if constexpr (REVERSE) {
-    s.mean_e = fold_partials<AddOP, 16>(real ? part.e : (P)0) * inv_n;
-    s.mean_eh = fold_partials<AddOP, 16>(real ? part.ex + by * part.e : (P)0) * inv_n * s.r;
-  }
-  return s;
-}
-template <bool REVERSE, class P>
-__device__ __forceinline__ NormStats<P> norm_alone(const NormPart<P>& part, P inv_n, P eps) {
-  NormStats<P> s;
-  s.pivot = part.pivot;
-  s.off = part.off * inv_n;
-  s.r = rsqrt_of(variance_of(part.square * inv_n, s.off) + eps);
-  if constexpr (REVERSE) {
-    s.mean_e = part.e * inv_n;
-    s.mean_eh = (part.ex - s.off * part.e) * inv_n * s.r;
-  }
-  return s;
-}
-
 constexpr int NORM_WAVES = NORM_BLOCK / WAVE;
 
-/* Half-precision rows are bound by arithmetic as much as by memory (13 instructions an element in the
- * forward when every operand is widened first), so products take their operands as stored:
- * a * b + c with a (and b) in half is one v_fma_mix_f32, exact in the product as fp32 is. */
+/* Half-precision rows are bound by arithmetic as much as by memory (23 vector instructions an element in
+ * the reverse, 19 us of the 39 a [16384, 2048] pass took, when every operand was widened first), so
+ * products take their operands as stored: a * b + c with a (and b) in half is one v_fma_mix_f32, and
+ * sums of elements and of products go two at a time through v_dot2_f32_f16, both with fp32 results. */
 __device__ __forceinline__ float mix_fma(_Float16 a, float b, float c) { return __builtin_fmaf((float)a, b, c); }
 __device__ __forceinline__ float mix_fma(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
 __device__ __forceinline__ double mix_fma(double a, double b, double c) { return __builtin_fma(a, b, c); }
-/* a - c; `one` is a one that the compiler does not know, or the half case would be two instructions again */
-__device__ __forceinline__ float mix_less(_Float16 a, float c, float one) { return __builtin_fmaf((float)a, one, -c); }
-__device__ __forceinline__ float mix_less(float a, float c, float) { return a - c; }
-__device__ __forceinline__ double mix_less(double a, double c, double) { return a - c; }
-__device__ __forceinline__ float mix_add(_Float16 a, float c, float one) { return __builtin_fmaf((float)a, one, c); }
-__device__ __forceinline__ float mix_add(float a, float c, float) { return a + c; }
-__device__ __forceinline__ double mix_add(double a, double c, double) { return a + c; }
+/* a - c and a + c; `one` is a one that the compiler does not know, or the half case would be two instructions again */
+template <class T, class P> __device__ __forceinline__ P mix_less(T a, P c, P one) {
+  if constexpr (sizeof(T) == 2) return __builtin_fmaf((float)a, one, -c);
+  else return a - c;
+}
+template <class T, class P> __device__ __forceinline__ P mix_add(T a, P c, P one) {
+  if constexpr (sizeof(T) == 2) return __builtin_fmaf((float)a, one, c);
+  else return a + c;
+}
 template <class T, class P> __device__ __forceinline__ P mix_mul(T a, T b) {
   if constexpr (sizeof(T) == 2) return __builtin_fmaf((float)a, (float)b, 0.0f);
   else return a * b;
 }
-__device__ __forceinline__ float norm_out(float h, float g, _Float16 b) { return __builtin_fmaf(h, g, (float)b); }
-__device__ __forceinline__ float norm_out(float h, float g, float b) { return __builtin_fmaf(h, g, b); }
-__device__ __forceinline__ double norm_out(double h, double g, double b) { return __builtin_fma(h, g, b); }
-/* the sum of a pack (two halves an instruction) */
-template <class T, int W, class P> __device__ __forceinline__ P pack_sum(const typename vec_of<T, W>::type& v) {
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+/* s + the sum of a pack's products with another's, or of its elements */
+template <int W, class V> __device__ __forceinline__ float half_dot(const V& a, const V& b, float s) {
+#pragma unroll
+  for (int i = 0; i < W; i += 2) s = __builtin_amdgcn_fdot2(half2_t{a[i], a[i + 1]}, half2_t{b[i], b[i + 1]}, s, false);
+  return s;
+}
+template <class T, int W, class P, class V> __device__ __forceinline__ P pack_sum(const V& v) {
   P s = (P)0;
   if constexpr (sizeof(T) == 2) {
-    typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
-    const half2_t ones = {(_Float16)1, (_Float16)1};
+    V ones;
 #pragma unroll
-    for (int i = 0; i < W; i += 2) s = __builtin_amdgcn_fdot2(half2_t{v[i], v[i + 1]}, ones, s, false);
+    for (int i = 0; i < W; ++i) ones[i] = (T)1;
+    s = half_dot<W>(v, ones, s);
   } else {
 #pragma unroll
     for (int i = 0; i < W; ++i) s += v[i];
@@ -272,206 +272,316 @@ template <class T, int W, class P> __device__ __forceinline__ P pack_sum(const t
   return s;
 }
 
+/* Several sums over the S lanes of a row at once. Two (four) values a lane become one after a step (two)
+ * of the butterfly, the even lanes going on with the first and the odd ones with the second (every
+ * fourth lane with one of four), which takes 19 instructions for four values instead of 48. Steps
+ * between lanes that agree in their lowest bits follow: rotations by 8 and 4 within 16 lanes, then the
+ * swaps of half wavefronts. Lane l ends with the sum of value l % 2 (l % 4). */
+constexpr int DPP_ROR4 = 0x124, DPP_ROR8 = 0x128;
+template <int S, class P> __device__ __forceinline__ P fold_apart(P v) {
+  static_assert(S == 16 || S == 32 || S == 64, "16, 32 or 64 lanes");
+  v += dpp_move<DPP_ROR8>(v);
+  v += dpp_move<DPP_ROR4>(v);
+  if constexpr (S >= 32) v = fold_swap16<AddOP>(v);
+  if constexpr (S >= 64) v = fold_swap32<AddOP>(v);
+  return v;
+}
+template <int S, class P> __device__ __forceinline__ P lanes_sum2(P a, P b) {
+  const bool odd = threadIdx.x & 1;
+  a += dpp_move<DPP_XOR1>(a);
+  b += dpp_move<DPP_XOR1>(b);
+  P v = odd ? b : a;
+  v += dpp_move<DPP_XOR2>(v);
+  return fold_apart<S>(v);
+}
+template <int S, class P> __device__ __forceinline__ P lanes_sum4(P a, P b, P c, P d) {
+  const bool odd = threadIdx.x & 1, high = threadIdx.x & 2;
+  a += dpp_move<DPP_XOR1>(a);
+  b += dpp_move<DPP_XOR1>(b);
+  c += dpp_move<DPP_XOR1>(c);
+  d += dpp_move<DPP_XOR1>(d);
+  P lo = odd ? b : a, hi = odd ? d : c;
+  lo += dpp_move<DPP_XOR2>(lo);
+  hi += dpp_move<DPP_XOR2>(hi);
+  return fold_apart<S>(high ? hi : lo);
+}
+/* value q of a lanes_sum2 or lanes_sum4 on all lanes: the q-th lane of every four */
+template <int Q, class P> __device__ __forceinline__ P quad_lane(P v) { return dpp_move<Q * 0x55>(v); }
+
+/* What the wavefronts of a row hand each other: a pivot near the mean of a wavefront's own elements, the
+ * sums of x - pivot (`off`) and its square, and in the reverse those of e = dy * gain and e * (x - pivot).
+ * Every wavefront takes its sums about a pivot of its own, so one exchange does for the mean and the
+ * variance, without a difference of squares of values far from zero. */
+enum { PART_OFF = 0, PART_SQUARE = 1, PART_E = 2, PART_EX = 3, PART_PIVOT = 4, PART_WORDS = 8 };
+template <class P> struct alignas(32) NormPart { P v[PART_WORDS]; };
+template <class P> struct NormStats {
+  P back; /* x - mean is (x - pivot) + back */
+  P r, mean_e, mean_eh;
+};
+
+/* A value of each of a row's wavefronts added up: lane i holds the (i % pow2)-th wavefront's, pow2 the next
+ * power of two from gw. */
+template <class P> __device__ __forceinline__ P waves_sum(P v, int gw) {
+  v += dpp_move<DPP_XOR1>(v);
+  if (gw > 2) v += dpp_move<DPP_XOR2>(v);
+  if (gw > 4) v += dpp_move<DPP_HALF_MIRROR>(v);
+  if (gw > 8) v += dpp_move<DPP_MIRROR>(v);
+  return v;
+}
+
+/* The row's statistics from the parts of its wavefronts, which lie in LDS behind a barrier. `held`: how many
+ * elements the wavefront of this lane's slot has (0 for a slot from gw on). All lanes get the same bits. */
+template <bool REVERSE, class P>
+__device__ __forceinline__ NormStats<P> norm_join(const NormPart<P>* parts, int slot, int gw, P held, P pivot, P inv_n, P eps) {
+  const bool real = slot < gw;
+  const NormPart<P>& part = parts[real ? slot : 0];
+  const P first = parts[0].v[PART_PIVOT], off = part.v[PART_OFF], apart = part.v[PART_PIVOT] - first;
+  NormStats<P> s;
+  const P mean = waves_sum(real ? off + held * apart : (P)0, gw) * inv_n; /* above the first wavefront's pivot */
+  const P by = apart - mean;                                             /* pivot - mean, for the slot's wavefront */
+  const P square = waves_sum(real ? part.v[PART_SQUARE] + by * ((P)2 * off + held * by) : (P)0, gw) * inv_n;
+  s.r = rsqrt_of((square < (P)0 ? (P)0 : square) + eps);
+  s.back = pivot - first - mean;
+  if constexpr (REVERSE) {
+    const P e = part.v[PART_E];
+    s.mean_e = waves_sum(real ? e : (P)0, gw) * inv_n;
+    s.mean_eh = waves_sum(real ? part.v[PART_EX] + by * e : (P)0, gw) * inv_n * s.r;
+  }
+  return s;
+}
+template <bool REVERSE, class P>
+__device__ __forceinline__ NormStats<P> norm_alone(P off, P square, P e, P ex, P inv_n, P eps) {
+  NormStats<P> s;
+  s.back = -off * inv_n;
+  s.r = rsqrt_of(variance_of(square * inv_n, s.back) + eps);
+  if constexpr (REVERSE) {
+    s.mean_e = e * inv_n;
+    s.mean_eh = (ex * inv_n + s.back * s.mean_e) * s.r;
+  }
+  return s;
+}
+
+/* The statistics of the row a wavefront has (part of) in registers. sum: of the elements `pivot_held` the pivot
+ * is the mean of, over the lanes already; measure(pivot) gives a lane's sums about it. Half-precision
+ * rows take their pivot from all elements: it is their mean as fp32 has it, and what its rounding leaves
+ * over is sum - held * pivot, so no second sum of differences is needed. The other types take it from
+ * a first pack a lane and add up the differences. */
+template <class T, int SUB, bool REVERSE, class P, class F>
+__device__ __forceinline__ NormStats<P> norm_stats(P sum, P inv_pivot_held, P held, P held_slot, int slot, int gw, NormPart<P>* slots, int mine,
+                                                   P inv_n, P eps, F&& measure) {
+  sum = lanes_allreduce<AddOP, SUB>(sum);
+  P pivot = sum * inv_pivot_held;
+  settle(pivot); /* rounded here: x - sum * inv in one step is not x minus what is handed on */
+  P off = (P)0, square = (P)0, e = (P)0, ex = (P)0;
+  measure(pivot, off, square, e, ex);
+  constexpr bool WHOLE = sizeof(T) == 2;
+  const bool alone = SUB < WAVE || gw == 1;
+  if constexpr (SUB == 8) {
+    off = WHOLE ? mix_fma((float)pivot, (float)-held, (float)sum) : lanes_allreduce<AddOP, SUB>(off);
+    square = lanes_allreduce<AddOP, SUB>(square);
+    if constexpr (REVERSE) {
+      e = lanes_allreduce<AddOP, SUB>(e);
+      ex = lanes_allreduce<AddOP, SUB>(ex);
+    }
+    return norm_alone<REVERSE>(off, square, e, ex, inv_n, eps);
+  } else {
+    P v;
+    if constexpr (REVERSE) v = lanes_sum4<SUB>(off, square, e, ex);
+    else if constexpr (WHOLE) v = lanes_allreduce<AddOP, SUB>(square);
+    else v = lanes_sum2<SUB>(off, square);
+    if constexpr (WHOLE) off = mix_fma((float)pivot, (float)-held, (float)sum);
+    if (alone) {
+      if constexpr (!WHOLE) off = quad_lane<PART_OFF>(v);
+      return norm_alone<REVERSE>(off, WHOLE && !REVERSE ? v : quad_lane<PART_SQUARE>(v), quad_lane<PART_E>(v), quad_lane<PART_EX>(v), inv_n, eps);
+    }
+    const int l = threadIdx.x % WAVE;
+    if (l <= PART_PIVOT) {
+      if (WHOLE && l == PART_OFF) v = off;
+      slots[mine].v[l] = l == PART_PIVOT ? pivot : v;
+    }
+    lds_barrier();
+    return norm_join<REVERSE>(slots, slot, gw, held_slot, pivot, inv_n, eps);
+  }
+}
+
+/* Where a thread of a launch belongs: rows_here rows a workgroup, held by G lanes each. SINGLE: one row a
+ * workgroup, held by all of it. */
+template <int SUB, bool SINGLE = false> struct NormPlace {
+  int G, rows_here, sub, base_wave, mine, slot;
+  __device__ __forceinline__ explicit NormPlace(int gw) {
+    G = SUB < WAVE ? SUB : SINGLE ? (int)blockDim.x : gw * WAVE;
+    rows_here = SINGLE ? 1 : (int)blockDim.x / G;
+    sub = SINGLE ? 0 : threadIdx.x / G;
+    base_wave = sub * gw;
+    mine = (int)threadIdx.x / WAVE - base_wave;
+    slot = threadIdx.x & (gw > 8 ? 15 : gw > 4 ? 7 : gw > 2 ? 3 : 1);
+  }
+};
+
 /* ------------------------------------------------------------------ forward */
 
-template <class T, int W, int SUB, int NV, bool LOOSE, bool PAIR>
+/* SUB <= 64: a wavefront or a part of one holds a row; SUB = ROW_A_BLOCK: the workgroup does. Once x - pivot
+ * is taken the registers of x are free again: a workgroup that walks several rows has the next row's
+ * loads on their way while this one is reduced and written. */
+constexpr int ROW_A_BLOCK = 1024;
+template <class T, int W, int SUB_, int NV, bool LOOSE, bool KEEP>
 __global__ __launch_bounds__(NORM_BLOCK) void layernorm_fwd_rows(
-    const T* x, const T* gain, const T* bias, T* y, typename precision<T>::type eps, size_t m, size_t n, int gw) {
+    const T* x, const T* gain, const T* bias, T* y, typename precision<T>::type eps, size_t m, size_t n) {
+  constexpr bool SINGLE = SUB_ == ROW_A_BLOCK;
+  constexpr int SUB = SINGLE ? WAVE : SUB_;
   using P = typename precision<T>::type;
   using Row = NormRow<T, W, SUB, NV, LOOSE>;
   using V = typename Row::V;
-  __shared__ NormPart<P> parts[2][NORM_WAVES];
-  const P inv_n = (P)1 / (P)n;
-  const int wave = threadIdx.x / WAVE, G = SUB < WAVE ? SUB : gw * WAVE;
-  const int rows_here = (int)blockDim.x / G, sub = threadIdx.x / G;
-  const int base_wave = sub * gw, mine = wave - base_wave; /* of the row's wavefronts */
-  const Row rw(n, G, threadIdx.x % G);
-  const P held = (P)rw.held(SUB < WAVE ? 0 : mine, n), inv_held = held > (P)0 ? (P)1 / held : (P)0;
-  const P held_slot = SUB < WAVE || gw == 1 ? held : (P)rw.held(threadIdx.x & 15, n);
+  constexpr int PIVOT_PACKS = sizeof(T) == 2 ? NV : 1;
+  __shared__ NormPart<P> parts[2][SINGLE ? NORM_WAVES : 1];
+  const int gw = SINGLE ? (int)blockDim.x / WAVE : 1;
+  const NormPlace<SUB, SINGLE> at(gw);
+  const Row rw(n, at.G, SINGLE ? (int)threadIdx.x : (int)threadIdx.x % SUB);
 
-  V gv[NV], bv[NV]; /* as stored, widened where they are used */
-  if (gain) rw.template fetch<false>(gain, gv);
-  else
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-      for (int i = 0; i < W; ++i) gv[k][i] = (T)1;
-  if (bias) rw.template fetch<false>(bias, bv);
-  else
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-      for (int i = 0; i < W; ++i) bv[k][i] = (T)0;
-
-  const size_t last = m - 1, stride = (size_t)gridDim.x * rows_here;
-  auto fetch = [&](V (&xs)[NV], size_t base) { /* a row beyond the last reads the last */
-    const size_t row = base + sub;
-    rw.template fetch<true>(x + (row < last ? row : last) * n, xs);
+  const size_t stride = (size_t)gridDim.x * at.rows_here;
+  size_t base = (size_t)blockIdx.x * at.rows_here;
+  auto fetch = [&](V (&xs)[NV], size_t from) { /* a row beyond the last reads the last */
+    const size_t row = from + at.sub, real = row < m ? row : m - 1;
+    rw.template fetch<KEEP>(x + real * n, xs, rw.ends(real, m, n));
   };
+  V xs[NV], gv[NV], bv[NV]; /* as stored, widened where they are used */
+  fetch(xs, base);
+  rw.fetch_vector(gain, gv, (T)1);
+  rw.fetch_vector(bias, bv, (T)0);
+  const P inv_n = (P)1 / (P)n;
+  const P held = (P)rw.held(at.mine, NV, n), pivot_held = (P)rw.held(at.mine, PIVOT_PACKS, n);
+  const P inv_pivot_held = pivot_held > (P)0 ? (P)1 / pivot_held : (P)0, held_slot = (P)rw.held(at.slot, NV, n);
   P one = (P)1;
   settle(one);
-  auto finish = [&](const V (&xs)[NV], size_t base, NormPart<P>* slots) {
+
+  int parity = 0;
+  for (; base < m; base += stride, parity ^= 1) {
+    rw.mask(xs);
     P s = (P)0;
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const P sk = pack_sum<T, W, P>(xs[k]); /* past the end of a cut pack: zeros */
+    for (int k = 0; k < PIVOT_PACKS; ++k) {
+      const P sk = pack_sum<T, W, P>(xs[k]);
       s += rw.inside(k) ? sk : (P)0;
     }
     P d[NV][W];
-    NormPart<P> part;
-    part.pivot = lanes_allreduce<AddOP, SUB>(s) * inv_held;
-    settle(part.pivot); /* rounded here: x - s * inv_held in one step is not x minus what is handed on */
-    part.off = part.square = (P)0;
+    const NormStats<P> st = norm_stats<T, SUB, false>(s, inv_pivot_held, held, held_slot, at.slot, gw, parts[parity], at.mine, inv_n, eps,
+                                                      [&](P pivot, P& off, P& square, P&, P&) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      P tk = (P)0, qk = (P)0;
+      for (int k = 0; k < NV; ++k) {
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        d[k][i] = mix_less(xs[k][i], part.pivot, one);
-        if constexpr (LOOSE) d[k][i] = i < rw.rp.valid(rw.pack(k)) ? d[k][i] : (P)0;
-        tk += d[k][i];
-        qk += d[k][i] * d[k][i];
+        for (int i = 0; i < W; ++i) d[k][i] = mix_less<T, P>(xs[k][i], pivot, one);
+        if (rw.cut(k))
+#pragma unroll
+          for (int i = 0; i < W; ++i) d[k][i] = i < rw.rp.last ? d[k][i] : (P)0;
       }
-      part.off += rw.inside(k) ? tk : (P)0;
-      part.square += rw.inside(k) ? qk : (P)0;
-    }
-    part.off = lanes_allreduce<AddOP, SUB>(part.off);
-    part.square = lanes_allreduce<AddOP, SUB>(part.square);
-    NormStats<P> st;
-    if (SUB < WAVE || gw == 1) {
-      st = norm_alone<false>(part, inv_n, eps);
-    } else {
-      if (threadIdx.x % WAVE == 0) slots[wave] = part;
-      lds_barrier();
-      st = norm_join<false>(slots + base_wave, gw, held_slot, inv_n, eps);
-    }
-    const P back = part.pivot - st.pivot - st.off; /* what x - mean is above d */
-    const size_t row = base + sub;
+      if (base + stride < m) fetch(xs, base + stride);
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        P tk = (P)0, qk = (P)0;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          if constexpr (sizeof(T) != 2) tk += d[k][i];
+          qk += d[k][i] * d[k][i];
+        }
+        off += rw.inside(k) ? tk : (P)0;
+        square += rw.inside(k) ? qk : (P)0;
+      }
+    });
+    const size_t row = base + at.sub;
     if (row < m) {
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
         if (rw.inside(k)) {
           P out[W];
 #pragma unroll
-          for (int i = 0; i < W; ++i) out[i] = norm_out(d[k][i] + back, mix_fma(gv[k][i], st.r, (P)0), bv[k][i]);
+          for (int i = 0; i < W; ++i) out[i] = (d[k][i] + st.back) * mix_fma(gv[k][i], st.r, (P)0) + (P)bv[k][i];
           rw.rp.store(y + row * n, rw.pack(k), out);
         }
       }
-    }
-  };
-
-  size_t base = (size_t)blockIdx.x * rows_here;
-  V ax[NV];
-  if constexpr (PAIR) { /* the next rows are on their way while these are reduced and written */
-    V bx[NV];
-    fetch(ax, base);
-    for (; base < m; base += 2 * stride) {
-      fetch(bx, base + stride);
-      __builtin_amdgcn_sched_barrier(0);
-      finish(ax, base, parts[0]);
-      fetch(ax, base + 2 * stride);
-      __builtin_amdgcn_sched_barrier(0);
-      finish(bx, base + stride, parts[1]);
-    }
-  } else {
-    int parity = 0;
-    for (; base < m; base += stride, parity ^= 1) {
-      fetch(ax, base);
-      finish(ax, base, parts[parity]);
     }
   }
 }
 
 /* ------------------------------------------------------------------ reverse */
 
-/* Persistent workgroups walk the rows; the next rows' x and dy are on their way while these are reduced
- * behind a barrier that orders LDS traffic only, and the columns' sums for dg and db stay in registers.
- * At the end the rows of a workgroup are folded in order and it leaves ONE partial row of 2n sums. */
-template <class T, int W, int SUB, int NV, bool BLEND, bool LOOSE, bool PAIR>
-__global__ __launch_bounds__(NORM_BLOCK) void layernorm_rev_rows(
+/* Persistent workgroups walk the rows; with PAIR the next rows' x and dy are on their way (into a second
+ * set of registers) while these are reduced, behind a barrier that orders LDS traffic only, and written.
+ * The columns' sums for dg and db stay in registers; at the end the rows of a workgroup are folded in
+ * order and it leaves ONE partial row of 2n sums. BLOCK 512 leaves a lane 256 registers. */
+template <class T, int W, int SUB, int NV, bool BLEND, bool LOOSE, bool PAIR, int BLOCK>
+__global__ __launch_bounds__(BLOCK) void layernorm_rev_rows(
     const T* x, const T* gain, const T* dy, T* dx, typename precision<T>::type* partials,
     typename precision<T>::type eps, typename precision<T>::type alpha, size_t m, size_t n, int gw) {
   using P = typename precision<T>::type;
   using Row = NormRow<T, W, SUB, NV, LOOSE>;
   using V = typename Row::V;
-  __shared__ NormPart<P> parts[2][NORM_WAVES];
-  __shared__ P comb[NORM_BLOCK * W];
+  constexpr int PIVOT_PACKS = sizeof(T) == 2 ? NV : 1;
+  constexpr int WAVES = BLOCK / WAVE;
+  __shared__ NormPart<P> parts[2][SUB < WAVE ? 1 : WAVES];
+  __shared__ P comb[BLOCK * W];
   const P inv_n = (P)1 / (P)n;
-  const int wave = threadIdx.x / WAVE, G = SUB < WAVE ? SUB : gw * WAVE;
-  const int rows_here = (int)blockDim.x / G, sub = threadIdx.x / G;
-  const int base_wave = sub * gw, mine = wave - base_wave;
-  const Row rw(n, G, threadIdx.x % G);
-  const P held = (P)rw.held(SUB < WAVE ? 0 : mine, n), inv_held = held > (P)0 ? (P)1 / held : (P)0;
-  const P held_slot = SUB < WAVE || gw == 1 ? held : (P)rw.held(threadIdx.x & 15, n);
+  const NormPlace<SUB> at(gw);
+  const Row rw(n, at.G, threadIdx.x % at.G);
+  const P held = (P)rw.held(at.mine, NV, n), pivot_held = (P)rw.held(at.mine, PIVOT_PACKS, n);
+  const P inv_pivot_held = pivot_held > (P)0 ? (P)1 / pivot_held : (P)0, held_slot = (P)rw.held(at.slot, NV, n);
+  P one = (P)1;
+  settle(one);
 
   V gv[NV];
-  if (gain) rw.template fetch<false>(gain, gv);
-  else
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-      for (int i = 0; i < W; ++i) gv[k][i] = (T)1;
+  rw.fetch_vector(gain, gv, (T)1);
   P acc_g[NV][W], acc_b[NV][W];
 #pragma unroll
   for (int k = 0; k < NV; ++k)
 #pragma unroll
     for (int i = 0; i < W; ++i) acc_g[k][i] = acc_b[k][i] = (P)0;
 
-  const size_t last = m - 1, stride = (size_t)gridDim.x * rows_here;
-  auto fetch = [&](V (&xs)[NV], V (&ds)[NV], size_t base) {
-    size_t row = base + sub;
-    row = row < last ? row : last;
-    rw.template fetch<true>(x + row * n, xs);
-    rw.template fetch<true>(dy + row * n, ds);
+  const size_t stride = (size_t)gridDim.x * at.rows_here;
+  auto fetch = [&](V (&xs)[NV], V (&ds)[NV], size_t base) { /* a row beyond the last reads the last */
+    const size_t row = base + at.sub, real = row < m ? row : m - 1;
+    const bool end = rw.ends(real, m, n);
+    rw.template fetch<false>(x + real * n, xs, end);
+    rw.template fetch<false>(dy + real * n, ds, end);
   };
-  P one = (P)1;
-  settle(one);
-  auto finish = [&](const V (&xs)[NV], const V (&ds)[NV], size_t base, NormPart<P>* slots) {
+  auto finish = [&](V (&xs)[NV], V (&ds)[NV], size_t base, NormPart<P>* slots) {
+    rw.mask(xs);
+    rw.mask(ds);
     P s = (P)0;
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const P sk = pack_sum<T, W, P>(xs[k]); /* past the end of a cut pack: zeros, as dy's */
+    for (int k = 0; k < PIVOT_PACKS; ++k) {
+      const P sk = pack_sum<T, W, P>(xs[k]);
       s += rw.inside(k) ? sk : (P)0;
     }
-    P t[NV][W], e[NV][W];
-    NormPart<P> part;
-    part.pivot = lanes_allreduce<AddOP, SUB>(s) * inv_held;
-    settle(part.pivot); /* rounded here: x - s * inv_held in one step is not x minus what is handed on */
-    part.off = part.square = part.e = part.ex = (P)0;
+    P t[NV][W];
+    const NormStats<P> st = norm_stats<T, SUB, true>(s, inv_pivot_held, held, held_slot, at.slot, gw, slots + (SUB < WAVE ? 0 : at.base_wave), at.mine,
+                                                     inv_n, eps, [&](P pivot, P& off, P& square, P& e, P& ex) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      P tk = (P)0, qk = (P)0, ek = (P)0, fk = (P)0;
+      for (int k = 0; k < NV; ++k) {
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        t[k][i] = mix_less(xs[k][i], part.pivot, one);
-        if constexpr (LOOSE) t[k][i] = i < rw.rp.valid(rw.pack(k)) ? t[k][i] : (P)0;
-        e[k][i] = mix_mul<T, P>(ds[k][i], gv[k][i]);
-        tk += t[k][i];
-        qk += t[k][i] * t[k][i];
-        ek += e[k][i];
-        fk += e[k][i] * t[k][i];
+        for (int i = 0; i < W; ++i) t[k][i] = mix_less<T, P>(xs[k][i], pivot, one);
+        if (rw.cut(k))
+#pragma unroll
+          for (int i = 0; i < W; ++i) t[k][i] = i < rw.rp.last ? t[k][i] : (P)0;
+        P tk = (P)0, qk = (P)0, ek = (P)0, fk = (P)0;
+        if constexpr (sizeof(T) == 2) ek = half_dot<W>(ds[k], gv[k], ek);
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          const P p = mix_mul<T, P>(ds[k][i], gv[k][i]);
+          if constexpr (sizeof(T) != 2) {
+            tk += t[k][i];
+            ek += p;
+          }
+          qk += t[k][i] * t[k][i];
+          fk += p * t[k][i];
+        }
+        const bool in = rw.inside(k);
+        off += in ? tk : (P)0;
+        square += in ? qk : (P)0;
+        e += in ? ek : (P)0;
+        ex += in ? fk : (P)0;
       }
-      const bool in = rw.inside(k);
-      part.off += in ? tk : (P)0;
-      part.square += in ? qk : (P)0;
-      part.e += in ? ek : (P)0;
-      part.ex += in ? fk : (P)0;
-    }
-    part.off = lanes_allreduce<AddOP, SUB>(part.off);
-    part.square = lanes_allreduce<AddOP, SUB>(part.square);
-    part.e = lanes_allreduce<AddOP, SUB>(part.e);
-    part.ex = lanes_allreduce<AddOP, SUB>(part.ex);
-    NormStats<P> st;
-    if (SUB < WAVE || gw == 1) {
-      st = norm_alone<true>(part, inv_n, eps);
-    } else {
-      if (threadIdx.x % WAVE == 0) slots[wave] = part;
-      lds_barrier();
-      st = norm_join<true>(slots + base_wave, gw, held_slot, inv_n, eps);
-    }
-    const P back = (part.pivot - st.pivot - st.off) * st.r; /* h = (x - mean) * r = t * r + back */
-    const P re = st.r * st.mean_e, rh = st.r * st.mean_eh;
-    const size_t row = base + sub;
+    });
+    const P back = st.back * st.r, re = st.r * st.mean_e, rh = st.r * st.mean_eh; /* h = (x - mean) * r = t * r + back */
+    const size_t row = base + at.sub;
     if (row < m) {
       T* out_row = dx + row * n;
 #pragma unroll
@@ -481,9 +591,9 @@ __global__ __launch_bounds__(NORM_BLOCK) void layernorm_rev_rows(
 #pragma unroll
           for (int i = 0; i < W; ++i) {
             const P h = t[k][i] * st.r + back;
-            out[i] = e[k][i] * st.r - re - h * rh;
+            out[i] = mix_mul<T, P>(ds[k][i], gv[k][i]) * st.r - re - h * rh;
             acc_g[k][i] = mix_fma(ds[k][i], h, acc_g[k][i]);
-            acc_b[k][i] = mix_add(ds[k][i], acc_b[k][i], one);
+            acc_b[k][i] = mix_add<T, P>(ds[k][i], acc_b[k][i], one);
           }
           if constexpr (BLEND) {
             P old[W];
@@ -497,7 +607,7 @@ __global__ __launch_bounds__(NORM_BLOCK) void layernorm_rev_rows(
     }
   };
 
-  size_t base = (size_t)blockIdx.x * rows_here;
+  size_t base = (size_t)blockIdx.x * at.rows_here;
   V ax[NV], ad[NV];
   if constexpr (PAIR) {
     V bx[NV], bd[NV];
@@ -521,8 +631,8 @@ __global__ __launch_bounds__(NORM_BLOCK) void layernorm_rev_rows(
   }
 
   /* the rows of a wavefront, then the row groups of the workgroup, a pack of every lane at a time */
-  const int groups = SUB < WAVE ? (int)blockDim.x / WAVE : rows_here;
-  const int width = SUB < WAVE ? SUB : G; /* lanes a group */
+  const int groups = SUB < WAVE ? (int)blockDim.x / WAVE : at.rows_here;
+  const int width = at.G; /* lanes a group */
   P* out = partials + (size_t)blockIdx.x * 2 * n;
 #pragma unroll
   for (int k = 0; k < NV; ++k)
@@ -544,11 +654,11 @@ __global__ __launch_bounds__(NORM_BLOCK) void layernorm_rev_rows(
         }
         continue;
       }
-      const int group = SUB < WAVE ? wave : sub, at = threadIdx.x % width;
+      const int group = SUB < WAVE ? (int)threadIdx.x / WAVE : at.sub, l = threadIdx.x % width;
       __syncthreads(); /* the sums before have been read */
       if (SUB == WAVE || threadIdx.x % WAVE < (unsigned)SUB)
 #pragma unroll
-        for (int i = 0; i < W; ++i) comb[(group * width + at) * W + i] = a[i];
+        for (int i = 0; i < W; ++i) comb[(group * width + l) * W + i] = a[i];
       __syncthreads();
       for (int c = threadIdx.x; c < width * W; c += blockDim.x) {
         const size_t col = (size_t)k * width * W + c;
@@ -621,59 +731,46 @@ template <class T> inline size_t layernorm_reverse_scratch_bytes(size_t m, size_
 }
 
 /* How a launch holds its rows: `sub` lanes a row below 64, else `gw` wavefronts, `nv` packs a lane, `rows`
- * rows a workgroup at a time, `per_cu` workgroups a compute unit that walk them (0: one workgroup for
- * every `rows` rows), `pair`: the next rows on their way while these are reduced. nv = 0: rows too long
- * for registers. */
+ * rows a workgroup at a time, `per_cu` workgroups a compute unit that walk them. nv = 0: rows too long for
+ * registers. The choices come from sweeps of all of these (interleaved repeats, launches on operands
+ * beyond the caches):
+ *   two packs a lane rather than one (r16 [4096, 8192] forward 24.3 us against 25.7, [16384, 2048] reverse 42.7
+ *   against 45.9) or four (27.2, 42.6), except where the workgroup would pass 16 wavefronts;
+ *   as many workgroups a unit as make 12 wavefronts of four-byte rows (r32 [4099, 5120] 29.9 us at ten, 30.6 at
+ *   twenty) and 20 of two-byte ones (r16 [8192, 2560] 16.6 at 18, 17.9 at 12, 18.5 at 30), whose lanes hold
+ *   half the bytes;
+ *   rows of more than 64 KiB, r16 rows of more than 32 KiB, read three times: what is left of the registers
+ *   spills (forward r32 [1024, 32768] 78 us against 87, r16 39 against 59). */
 struct NormPlan {
   int sub, nv, gw, rows, per_cu;
-  bool pair;
 };
 inline unsigned norm_grid(const NormPlan& p, size_t m) {
   const size_t need = (m + p.rows - 1) / p.rows, cap = (size_t)compute_units() * p.per_cu;
-  require(need < 0x7fffffffull || p.per_cu, "layernorm: too many rows for one grid");
-  return (unsigned)(p.per_cu && cap < need ? cap : need);
+  return (unsigned)(cap < need ? cap : need);
 }
 inline unsigned norm_block(const NormPlan& p) { return (unsigned)(p.rows * (p.sub < WAVE ? p.sub : p.gw * WAVE)); }
+inline int norm_waves(size_t packs, int nv) { return (int)((packs + (size_t)nv * WAVE - 1) / ((size_t)nv * WAVE)); }
 
 template <class T> inline NormPlan layernorm_forward_plan(size_t packs) {
-  constexpr int MAXNV = sizeof(T) == 2 ? 4 : 8;
-  if (packs <= 8) return {8, 1, 1, 32, 0, false};
-  if (packs <= 16) return {16, 1, 1, 16, 0, false};
-  if (packs <= 32) return {32, 1, 1, 8, 0, false};
-  for (int nv = 1; nv <= MAXNV; nv *= 2)
-    if (packs <= (size_t)nv * NORM_BLOCK) {
-      const int gw = (int)((packs + (size_t)nv * WAVE - 1) / ((size_t)nv * WAVE));
-      const int rows = NORM_WAVES / gw;
-      return {WAVE, nv, gw, rows, 2, false};
-    }
-  return {WAVE, 0, 0, 0, 0, false};
+  if (packs <= 8) return {8, 1, 1, 64, 4};
+  if (packs <= 16) return {16, 1, 1, 32, 4};
+  if (packs <= 32) return {32, 1, 1, 16, 4};
+  if (packs <= 64) return {WAVE, 1, 1, 8, 4};
+  if (packs <= 128) return {WAVE, 2, 1, 8, 3};
+  const int nv = packs <= 1024 || sizeof(T) == 2 ? 2 : 4, gw = norm_waves(packs, nv), waves = sizeof(T) == 2 ? 20 : 12;
+  if (gw > NORM_WAVES) return {WAVE, 0, 0, 0, 0};
+  return {WAVE, nv, gw, 1, waves / gw ? waves / gw : 1};
 }
 template <class T> inline NormPlan layernorm_reverse_plan(size_t packs) {
-  constexpr int MAXNV = sizeof(T) == 2 ? 2 : 4;
-  if (packs <= 8) return {8, 1, 1, 128, 1, true};
-  if (packs <= 16) return {16, 1, 1, 64, 1, true};
-  if (packs <= 32) return {32, 1, 1, 32, 1, true};
-  for (int nv = 1; nv <= MAXNV; nv *= 2)
-    if (packs <= (size_t)nv * NORM_BLOCK) {
-      const int gw = (int)((packs + (size_t)nv * WAVE - 1) / ((size_t)nv * WAVE));
-      return {WAVE, nv, gw, NORM_WAVES / gw, 1, nv == 1};
-    }
-  return {WAVE, 0, 0, 0, 0, false};
-}
-
-/* f.template operator()<SUB, NV, PAIR>() for a plan in registers */
-template <int MAXNV, class F> inline void for_norm_plan(const NormPlan& p, F&& f) {
-  auto at = [&]<int SUB, int NV>() {
-    if (p.pair) f.template operator()<SUB, NV, true>();
-    else f.template operator()<SUB, NV, false>();
-  };
-  if (p.sub == 8) at.template operator()<8, 1>();
-  else if (p.sub == 16) at.template operator()<16, 1>();
-  else if (p.sub == 32) at.template operator()<32, 1>();
-  else if (p.nv == 1) at.template operator()<WAVE, 1>();
-  else if (p.nv == 2) at.template operator()<WAVE, 2>();
-  else if (p.nv == 4) { if constexpr (MAXNV >= 4) at.template operator()<WAVE, 4>(); }
-  else { if constexpr (MAXNV >= 8) at.template operator()<WAVE, 8>(); }
+  if (packs <= 8) return {8, 1, 1, 64, 2};
+  if (packs <= 16) return {16, 1, 1, 32, 2};
+  if (packs <= 32) return {32, 1, 1, 16, 2};
+  if (packs <= 64) return {WAVE, 1, 1, 16, 1};
+  /* r16 rows of more than 24 KiB: four packs a lane and no more than eight wavefronts, which leaves room for the
+   * next row ([2048, 16384] 55.6 -> 52.5 us) */
+  const int nv = packs <= (sizeof(T) == 2 ? 1536 : 2048) ? 2 : 4, gw = norm_waves(packs, nv), rows = gw < 8 ? 8 / gw : 1;
+  if (gw > NORM_WAVES) return {WAVE, 0, 0, 0, 0};
+  return {WAVE, nv, gw, rows, sizeof(T) == 2 && nv == 2 && gw > 1 && gw <= 8 ? 2 : 1};
 }
 
 template <class T>
@@ -681,6 +778,8 @@ inline void layernorm_forward_as(const NormPlan& plan, const T* x, const T* gain
   using P = typename precision<T>::type;
   constexpr int W = PACK_BYTES / (int)sizeof(T);
   const bool loose = !(aligned16(x) && aligned16(y) && (!gain || aligned16(gain)) && (!bias || aligned16(bias)) && n % W == 0);
+  /* as RMSNorm's forward: the reverse reads x again */
+  const bool keep = keep_input(m * n * sizeof(T));
   if (plan.nv == 0) {
     const size_t cap = (size_t)compute_units() * 2;
     const dim3 grid((unsigned)(m < cap ? m : cap)), block(STREAM_THREADS);
@@ -688,10 +787,21 @@ inline void layernorm_forward_as(const NormPlan& plan, const T* x, const T* gain
     else layernorm_fwd_stream<T, W, false><<<grid, block, 0, stream>>>(x, gain, bias, y, (P)eps, m, n);
   } else {
     const dim3 grid(norm_grid(plan, m)), block(norm_block(plan));
-    for_norm_plan<sizeof(T) == 2 ? 4 : 8>(plan, [&]<int SUB, int NV, bool PAIR>() {
-      if (loose) layernorm_fwd_rows<T, W, SUB, NV, true, PAIR><<<grid, block, 0, stream>>>(x, gain, bias, y, (P)eps, m, n, plan.gw);
-      else layernorm_fwd_rows<T, W, SUB, NV, false, PAIR><<<grid, block, 0, stream>>>(x, gain, bias, y, (P)eps, m, n, plan.gw);
-    });
+    auto go = [&]<int SUB, int NV>() {
+      auto kept = [&]<bool KEEP>() {
+        if (loose) layernorm_fwd_rows<T, W, SUB, NV, true, KEEP><<<grid, block, 0, stream>>>(x, gain, bias, y, (P)eps, m, n);
+        else layernorm_fwd_rows<T, W, SUB, NV, false, KEEP><<<grid, block, 0, stream>>>(x, gain, bias, y, (P)eps, m, n);
+      };
+      if (keep) kept.template operator()<true>();
+      else kept.template operator()<false>();
+    };
+    if (plan.sub == 8) go.template operator()<8, 1>();
+    else if (plan.sub == 16) go.template operator()<16, 1>();
+    else if (plan.sub == 32) go.template operator()<32, 1>();
+    else if (plan.nv == 1) go.template operator()<WAVE, 1>();
+    else if (plan.gw == 1) go.template operator()<WAVE, 2>();
+    else if (plan.nv == 2) go.template operator()<ROW_A_BLOCK, 2>();
+    else if constexpr (sizeof(T) != 2) go.template operator()<ROW_A_BLOCK, 4>();
   }
   MP_CHECK_LAUNCH();
 }
@@ -725,13 +835,27 @@ inline void layernorm_reverse_as(const NormPlan& plan, const T* x, const T* gain
       rows = norm_grid(plan, m);
       require(rows <= layernorm_partial_rows(m), "layernorm reverse: more partial rows than the workspace holds");
       const dim3 grid((unsigned)rows), block(norm_block(plan));
-      for_norm_plan<sizeof(T) == 2 ? 2 : 4>(plan, [&]<int SUB, int NV, bool PAIR>() {
-        auto go = [&]<bool BLEND, bool LOOSE>() {
-          layernorm_rev_rows<T, W, SUB, NV, BLEND, LOOSE, PAIR><<<grid, block, 0, stream>>>(x, gain, dy, dx, partials, (P)eps, (P)alpha, m, n, plan.gw);
+      auto go = [&]<int SUB, int NV, bool PAIR, int BLOCK>() {
+        auto as = [&]<bool BLEND, bool LOOSE>() {
+          layernorm_rev_rows<T, W, SUB, NV, BLEND, LOOSE, PAIR, BLOCK><<<grid, block, 0, stream>>>(x, gain, dy, dx, partials, (P)eps, (P)alpha, m, n, plan.gw);
         };
-        if (alpha != 0.0) { if (loose) go.template operator()<true, true>(); else go.template operator()<true, false>(); }
-        else { if (loose) go.template operator()<false, true>(); else go.template operator()<false, false>(); }
-      });
+        if (alpha != 0.0) { if (loose) as.template operator()<true, true>(); else as.template operator()<true, false>(); }
+        else { if (loose) as.template operator()<false, true>(); else as.template operator()<false, false>(); }
+      };
+      /* the next rows' loads in flight where the registers hold them (r32 [8192, 4096] 70.6 us against 73.4
+       * without; r16 at two packs a lane spills and loses by it, 45.9 against 42.7) */
+      if (plan.sub == 8) go.template operator()<8, 1, false, 512>();
+      else if (plan.sub == 16) go.template operator()<16, 1, false, 512>();
+      else if (plan.sub == 32) go.template operator()<32, 1, false, 512>();
+      else if (plan.nv == 1) go.template operator()<WAVE, 1, false, 1024>();
+      else if (plan.nv == 2) {
+        if constexpr (sizeof(T) != 2) go.template operator()<WAVE, 2, true, 1024>();
+        else if (block.x <= 512) go.template operator()<WAVE, 2, false, 512>();
+        else go.template operator()<WAVE, 2, false, 1024>();
+      } else {
+        if constexpr (sizeof(T) == 2) { if (block.x <= 512) go.template operator()<WAVE, 4, true, 512>(); else go.template operator()<WAVE, 4, false, 1024>(); }
+        else go.template operator()<WAVE, 4, false, 1024>();
+      }
     }
     MP_CHECK_LAUNCH();
   }
