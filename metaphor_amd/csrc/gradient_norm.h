@@ -7,9 +7,15 @@
  * overflow or vanish, and in a fixed order, so the norm does not change from run to run. The norm is a
  * double on the device; nothing waits for the host.
  *
- * The tensors' addresses and sizes travel as kernel arguments, NORM_TENSORS of them a launch: nothing
- * is copied to the device and a captured launch keeps its own table. A table's work is cut into pieces of
- * NORM_PIECE bytes that the workgroups take in turn; each leaves one partial sum in the workspace.
+ * Tensors that lie one behind the other (a bucket of gradients) are walked as one run. The runs' addresses
+ * and sizes travel as kernel arguments, NORM_RUNS of them a launch: nothing is copied to the device and a
+ * captured launch keeps its own table. A table's work is cut into pieces of NORM_PIECE bytes, four 16-byte
+ * packs a thread; workgroups take them in turn for the squares, each leaving one partial sum in the
+ * workspace, and one each for the scaling.
+ *
+ * The squares are bound by reading the tensors once, the scaling by reading and writing them once. The
+ * squares read through loads that leave their end in the 256 MiB memory-side cache, and the scaling walks
+ * from that end backwards.
  */
 #ifndef MP_GRADIENT_NORM_H
 #define MP_GRADIENT_NORM_H
@@ -20,28 +26,43 @@
 
 namespace mp {
 
-constexpr int NORM_TENSORS = 96, NORM_THREADS = 256;
-constexpr size_t NORM_PIECE = 16384, NORM_PARTIALS = 2048;
+constexpr int NORM_RUNS = 120, NORM_THREADS = 256, NORM_PACKS = 4;
+constexpr size_t NORM_PIECE = (size_t)NORM_THREADS * NORM_PACKS * PACK_BYTES, NORM_PARTIALS = 2048;
+/* up to so many pieces the scaling adds up the partial sums itself, in every workgroup, and one launch is
+ * saved; beyond, a workgroup would spend as long on that as on its piece */
+constexpr size_t NORM_FUSED_PIECES = 1024;
 
 template <class T> struct NormTable {
-  const T* src[NORM_TENSORS];
-  T* dst[NORM_TENSORS];
-  unsigned long long size[NORM_TENSORS];
-  unsigned first[NORM_TENSORS + 1]; /* the number of the tensor's first piece; [count] is the end */
+  const T* src[NORM_RUNS];
+  T* dst[NORM_RUNS];
+  unsigned long long size[NORM_RUNS];
+  unsigned first[NORM_RUNS + 1]; /* the number of the run's first piece; [count] is the end */
   int count;
 };
 
-/* The tensor that piece `q` belongs to: the last one whose first piece is not behind it. Tensors of no
- * elements have no piece. */
-template <class T> __device__ __forceinline__ int norm_tensor_of(const NormTable<T>& t, unsigned q) {
-  int lo = 0, hi = t.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (t.first[mid] <= q) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
+/* The run that piece `q` belongs to: the last one whose first piece is not behind it. Runs have a piece at
+ * least. Every lane looks at two of the first pieces, so the search is one load and a vote. */
+template <class T> __device__ __forceinline__ int norm_run_of(const NormTable<T>& t, unsigned q) {
+  static_assert(NORM_RUNS <= 2 * WAVE, "two runs a lane");
+  const int lane = threadIdx.x % WAVE;
+  const bool lo = lane < t.count && t.first[lane] <= q, hi = lane + WAVE < t.count && t.first[lane + WAVE < NORM_RUNS ? lane + WAVE : 0] <= q;
+  return __popcll(__ballot(lo)) + __popcll(__ballot(hi)) - 1;
 }
+
+/* A piece's packs in registers: f(pack index u, offset, elements that exist). */
+template <class T> struct NormPiece {
+  static constexpr int W = PACK_BYTES / (int)sizeof(T);
+  static constexpr size_t LEN = NORM_PIECE / sizeof(T);
+  int run;
+  size_t lo, left; /* the piece's first element in its run, and the run's elements from there on */
+  __device__ __forceinline__ NormPiece(const NormTable<T>& t, unsigned q) {
+    run = norm_run_of(t, q);
+    lo = (size_t)(q - t.first[run]) * LEN;
+    left = t.size[run] - lo;
+  }
+  __device__ __forceinline__ size_t at(int u) const { return ((size_t)u * NORM_THREADS + threadIdx.x) * W; }
+  __device__ __forceinline__ bool whole() const { return left >= LEN; }
+};
 
 /* Sum over the workgroup's threads; every thread gets it. */
 __device__ __forceinline__ double norm_block_sum(double s, double* slots) {
@@ -55,23 +76,23 @@ __device__ __forceinline__ double norm_block_sum(double s, double* slots) {
 }
 
 template <class T> __global__ __launch_bounds__(NORM_THREADS) void gradient_squares(NormTable<T> t, double* partials) {
-  constexpr int W = PACK_BYTES / (int)sizeof(T);
-  constexpr size_t PIECE = NORM_PIECE / sizeof(T);
+  constexpr int W = NormPiece<T>::W;
+  using VL = typename loose_vec_of<T, W>::type;
   __shared__ double slots[NORM_THREADS / WAVE];
   double s = 0.0;
   for (unsigned q = blockIdx.x; q < t.first[t.count]; q += gridDim.x) {
-    const int k = norm_tensor_of(t, q);
-    const size_t lo = (size_t)(q - t.first[k]) * PIECE, size = t.size[k], hi = lo + PIECE < size ? lo + PIECE : size;
-    const T* src = t.src[k];
-    for (size_t i = lo + (size_t)threadIdx.x * W; i < hi; i += NORM_THREADS * W) {
-      if (i + W <= hi) {
-        double v[W];
-        load_pack_loose<T, W>(src + i, v);
+    const NormPiece<T> piece(t, q);
+    const T* src = t.src[piece.run] + piece.lo;
+    if (piece.whole()) {
+      typename vec_of<T, W>::type v[NORM_PACKS];
 #pragma unroll
-        for (int j = 0; j < W; ++j) s += v[j] * v[j];
-      } else {
-        for (size_t j = i; j < hi; ++j) s += (double)src[j] * (double)src[j];
-      }
+      for (int u = 0; u < NORM_PACKS; ++u) v[u] = *reinterpret_cast<const VL*>(src + piece.at(u));
+#pragma unroll
+      for (int u = 0; u < NORM_PACKS; ++u)
+#pragma unroll
+        for (int j = 0; j < W; ++j) s += (double)v[u][j] * (double)v[u][j];
+    } else {
+      for (size_t i = threadIdx.x; i < piece.left; i += NORM_THREADS) s += (double)src[i] * (double)src[i];
     }
   }
   s = norm_block_sum(s, slots);
@@ -94,57 +115,99 @@ static __global__ __launch_bounds__(NORM_THREADS) void gradient_norm_finish(cons
   }
 }
 
-template <class T> __global__ __launch_bounds__(NORM_THREADS) void gradient_scaled(NormTable<T> t, const double* norm, double max_norm) {
+/* FUSED: norm_in is what the squares left, `partials` sums; the first workgroup writes the norm. */
+template <class T, bool FUSED>
+__global__ __launch_bounds__(NORM_THREADS) void gradient_scaled(NormTable<T> t, const double* norm_in, unsigned partials, double* norm_out, double max_norm) {
   using P = typename precision<T>::type;
-  constexpr int W = PACK_BYTES / (int)sizeof(T);
-  constexpr size_t PIECE = NORM_PIECE / sizeof(T);
-  const double total = norm[0];
-  const P factor = total <= max_norm ? (P)1 : (P)(max_norm / total);
-  for (unsigned q = blockIdx.x; q < t.first[t.count]; q += gridDim.x) {
-    const int k = norm_tensor_of(t, q);
-    const size_t lo = (size_t)(q - t.first[k]) * PIECE, size = t.size[k], hi = lo + PIECE < size ? lo + PIECE : size;
-    const T* src = t.src[k];
-    T* dst = t.dst[k];
-    if (src == dst && total <= max_norm) continue; /* nothing to do in place */
-    for (size_t i = lo + (size_t)threadIdx.x * W; i < hi; i += NORM_THREADS * W) {
-      if (i + W <= hi) {
-        P v[W];
-        load_pack_loose<T, W>(src + i, v);
+  constexpr int W = NormPiece<T>::W;
+  using VL = typename loose_vec_of<T, W>::type;
+  const NormPiece<T> piece(t, t.first[t.count] - 1 - blockIdx.x); /* what was read last comes first */
+  const T* src = t.src[piece.run] + piece.lo;
+  T* dst = t.dst[piece.run] + piece.lo;
+  typename vec_of<T, W>::type v[NORM_PACKS];
+  const bool whole = piece.whole();
+  if (whole)
 #pragma unroll
-        for (int j = 0; j < W; ++j) v[j] *= factor;
-        store_pack_nt_loose<T, W>(dst + i, v);
-      } else {
-        for (size_t j = i; j < hi; ++j) dst[j] = (T)((P)src[j] * factor);
-      }
+    for (int u = 0; u < NORM_PACKS; ++u) v[u] = __builtin_nontemporal_load(reinterpret_cast<const VL*>(src + piece.at(u)));
+  double total;
+  if constexpr (FUSED) {
+    __shared__ double slots[NORM_THREADS / WAVE];
+    total = ::sqrt(norm_of(norm_in, partials, slots));
+    if (blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = total;
+  } else {
+    total = norm_in[0];
+  }
+  const bool within = total <= max_norm;
+  if (src == dst && within) return; /* nothing to do in place */
+  const P factor = within ? (P)1 : (P)(max_norm / total);
+  if (whole) {
+#pragma unroll
+    for (int u = 0; u < NORM_PACKS; ++u) {
+      P out[W];
+#pragma unroll
+      for (int j = 0; j < W; ++j) out[j] = (P)v[u][j] * factor;
+      store_pack_nt_loose<T, W>(dst + piece.at(u), out);
     }
+  } else {
+    for (size_t i = threadIdx.x; i < piece.left; i += NORM_THREADS) dst[i] = (T)((P)src[i] * factor);
   }
 }
 
 /* ------------------------------------------------------------------ host dispatch */
 
-/* f(table, pieces) for the tensors in groups of NORM_TENSORS. */
-template <class T, class F>
-inline void for_norm_tables(const void* const* grads, const void* const* outs, const len_t* sizes, size_t count, F&& f) {
-  constexpr size_t PIECE = NORM_PIECE / sizeof(T);
-  for (size_t base = 0; base < count; base += NORM_TENSORS) {
-    NormTable<T> t;
-    t.count = (int)(count - base < (size_t)NORM_TENSORS ? count - base : (size_t)NORM_TENSORS);
-    size_t pieces = 0;
-    for (int k = 0; k < t.count; ++k) {
-      t.src[k] = static_cast<const T*>(grads[base + k]);
-      t.dst[k] = outs ? const_cast<T*>(static_cast<const T*>(outs[base + k])) : nullptr;
-      t.size[k] = sizes[base + k];
-      t.first[k] = (unsigned)pieces;
-      pieces += (t.size[k] + PIECE - 1) / PIECE;
+/* The tensors as runs of neighbours: f(first tensor, elements) for each; a run goes on while the next
+ * tensor begins where the last one ended, in grads and, where there are any, in outs. */
+template <class T, class F> inline void for_norm_runs(const void* const* grads, const void* const* outs, const len_t* sizes, size_t count, F&& f) {
+  size_t k = 0;
+  while (k < count) {
+    if (sizes[k] == 0) {
+      ++k;
+      continue;
     }
-    t.first[t.count] = (unsigned)pieces;
-    f(t, (unsigned)pieces);
+    const size_t begin = k;
+    size_t size = 0;
+    auto follows = [&](const void* const* a) { return static_cast<const char*>(a[k]) == static_cast<const char*>(a[begin]) + size * sizeof(T); };
+    do {
+      size += sizes[k++];
+      while (k < count && sizes[k] == 0) ++k;
+    } while (k < count && follows(grads) && (!outs || follows(outs)));
+    f(begin, size);
   }
 }
 
-inline size_t norm_tables(size_t count) { return (count + NORM_TENSORS - 1) / NORM_TENSORS; }
+struct NormWork { size_t runs, pieces; };
+template <class T> inline NormWork norm_work(const void* const* grads, const void* const* outs, const len_t* sizes, size_t count) {
+  NormWork w{0, 0};
+  for_norm_runs<T>(grads, outs, sizes, count, [&](size_t, size_t size) {
+    ++w.runs;
+    w.pieces += (size * sizeof(T) + NORM_PIECE - 1) / NORM_PIECE;
+  });
+  return w;
+}
 
-/* Partial sums a table may leave: all of them are added by one workgroup. */
+/* f(table) for the runs in groups of NORM_RUNS */
+template <class T, class F>
+inline void for_norm_tables(const void* const* grads, const void* const* outs, const len_t* sizes, size_t count, F&& f) {
+  NormTable<T> t;
+  t.count = 0;
+  t.first[0] = 0;
+  for_norm_runs<T>(grads, outs, sizes, count, [&](size_t k, size_t size) {
+    t.src[t.count] = static_cast<const T*>(grads[k]);
+    t.dst[t.count] = outs ? const_cast<T*>(static_cast<const T*>(outs[k])) : nullptr;
+    t.size[t.count] = size;
+    const size_t pieces = (size * sizeof(T) + NORM_PIECE - 1) / NORM_PIECE;
+    t.first[t.count + 1] = t.first[t.count] + (unsigned)pieces;
+    if (++t.count == NORM_RUNS) {
+      f(t);
+      t.count = 0;
+    }
+  });
+  if (t.count) f(t);
+}
+
+/* Partial sums a table of so many tensors may leave: all of them are added by one workgroup. Tensors that
+ * form runs make fewer tables than they might, never more. */
+inline size_t norm_tables(size_t count) { return (count + NORM_RUNS - 1) / NORM_RUNS; }
 inline size_t norm_partials(size_t count) {
   const size_t each = NORM_PARTIALS / (norm_tables(count) ? norm_tables(count) : 1);
   return each < 64 ? 64 : each;
@@ -180,12 +243,11 @@ inline void gradient_check_limit(const void* outs, double max_norm, size_t count
 
 /* returns how many partial sums there are */
 template <class T>
-inline unsigned gradient_squares_all(const void* grads, const void* sizes, void* scratch, size_t count, hipStream_t stream) {
-  double* partials = static_cast<double*>(scratch);
+inline unsigned gradient_squares_all(const void* const* grads, const len_t* sizes, double* partials, size_t count, hipStream_t stream) {
   unsigned used = 0;
-  for_norm_tables<T>(static_cast<const void* const*>(grads), nullptr, static_cast<const len_t*>(sizes), count, [&](const NormTable<T>& t, unsigned pieces) {
-    if (pieces == 0) return;
-    const unsigned cap = (unsigned)norm_partials(count), blocks = pieces < cap ? pieces : cap;
+  const unsigned cap = (unsigned)norm_partials(norm_work<T>(grads, nullptr, sizes, count).runs);
+  for_norm_tables<T>(grads, nullptr, sizes, count, [&](const NormTable<T>& t) {
+    const unsigned pieces = t.first[t.count], blocks = pieces < cap ? pieces : cap;
     gradient_squares<T><<<dim3(blocks), dim3(NORM_THREADS), 0, stream>>>(t, partials + used);
     MP_CHECK_LAUNCH();
     used += blocks;
@@ -194,19 +256,12 @@ inline unsigned gradient_squares_all(const void* grads, const void* sizes, void*
 }
 
 template <class T>
-inline void gradient_norm_enqueue(const void* grads, const void* sizes, void* norm, void* scratch, double alpha, size_t count, hipStream_t stream) {
-  const unsigned used = gradient_squares_all<T>(grads, sizes, scratch, count, stream);
-  gradient_norm_finish<<<dim3(1), dim3(NORM_THREADS), 0, stream>>>(static_cast<const double*>(scratch), used, alpha, static_cast<double*>(norm));
-  MP_CHECK_LAUNCH();
-}
-
-template <class T>
-inline void gradient_scale_enqueue(const void* grads, const void* outs, const void* sizes, const void* norm, double max_norm, size_t count,
-                                   hipStream_t stream) {
-  for_norm_tables<T>(static_cast<const void* const*>(grads), static_cast<const void* const*>(outs), static_cast<const len_t*>(sizes), count,
-                     [&](const NormTable<T>& t, unsigned pieces) {
-    if (pieces == 0) return;
-    gradient_scaled<T><<<dim3(pieces), dim3(NORM_THREADS), 0, stream>>>(t, static_cast<const double*>(norm), max_norm);
+inline void gradient_scale_all(const void* const* grads, const void* const* outs, const len_t* sizes, const double* norm_in, unsigned partials, double* norm_out,
+                               double max_norm, size_t count, hipStream_t stream) {
+  for_norm_tables<T>(grads, outs, sizes, count, [&](const NormTable<T>& t) {
+    const dim3 grid(t.first[t.count]), block(NORM_THREADS);
+    if (norm_out) gradient_scaled<T, true><<<grid, block, 0, stream>>>(t, norm_in, partials, norm_out, max_norm);
+    else gradient_scaled<T, false><<<grid, block, 0, stream>>>(t, norm_in, 0, nullptr, max_norm);
     MP_CHECK_LAUNCH();
   });
 }
@@ -215,14 +270,18 @@ template <class T>
 inline void gradient_norm(const void* grads, const void* sizes, void* norm, void* scratch, double alpha, size_t count, hipStream_t stream) {
   gradient_check<T>(grads, nullptr, sizes, norm, count);
   gradient_check_scratch(scratch, count);
-  gradient_norm_enqueue<T>(grads, sizes, norm, scratch, alpha, count, stream);
+  double* partials = static_cast<double*>(scratch);
+  const unsigned used = gradient_squares_all<T>(static_cast<const void* const*>(grads), static_cast<const len_t*>(sizes), partials, count, stream);
+  gradient_norm_finish<<<dim3(1), dim3(NORM_THREADS), 0, stream>>>(partials, used, alpha, static_cast<double*>(norm));
+  MP_CHECK_LAUNCH();
 }
 
 template <class T>
 inline void gradient_scale(const void* grads, const void* outs, const void* sizes, const void* norm, double max_norm, size_t count, hipStream_t stream) {
   gradient_check_limit(outs, max_norm, count);
   gradient_check<T>(grads, outs, sizes, norm, count);
-  gradient_scale_enqueue<T>(grads, outs, sizes, norm, max_norm, count, stream);
+  gradient_scale_all<T>(static_cast<const void* const*>(grads), static_cast<const void* const*>(outs), static_cast<const len_t*>(sizes),
+                        static_cast<const double*>(norm), 0, nullptr, max_norm, count, stream);
 }
 
 template <class T>
@@ -231,8 +290,18 @@ inline void gradient_clip(const void* grads, const void* outs, const void* sizes
   gradient_check_limit(outs, max_norm, count);
   gradient_check<T>(grads, outs, sizes, norm, count);
   gradient_check_scratch(scratch, count);
-  gradient_norm_enqueue<T>(grads, sizes, norm, scratch, 0.0, count, stream);
-  gradient_scale_enqueue<T>(grads, outs, sizes, norm, max_norm, count, stream);
+  const void* const* src = static_cast<const void* const*>(grads);
+  const void* const* dst = static_cast<const void* const*>(outs);
+  const len_t* lengths = static_cast<const len_t*>(sizes);
+  double *partials = static_cast<double*>(scratch), *out = static_cast<double*>(norm);
+  const unsigned used = gradient_squares_all<T>(src, lengths, partials, count, stream);
+  const NormWork work = norm_work<T>(src, dst, lengths, count);
+  const bool fused = used > 0 && work.runs <= (size_t)NORM_RUNS && work.pieces <= NORM_FUSED_PIECES;
+  if (!fused) {
+    gradient_norm_finish<<<dim3(1), dim3(NORM_THREADS), 0, stream>>>(partials, used, 0.0, out);
+    MP_CHECK_LAUNCH();
+  }
+  gradient_scale_all<T>(src, dst, lengths, fused ? partials : out, used, fused ? out : nullptr, max_norm, count, stream);
 }
 
 }  // namespace mp
