@@ -13,9 +13,11 @@
  * packs a thread; workgroups take them in turn for the squares, each leaving one partial sum in the
  * workspace, and one each for the scaling.
  *
- * The squares are bound by reading the tensors once, the scaling by reading and writing them once. The
- * squares read through loads that leave their end in the 256 MiB memory-side cache, and the scaling walks
- * from that end backwards.
+ * The squares are bound by reading the tensors once, the scaling by reading and writing them once. r32,
+ * 203 M elements: squares 124 us (6.6 TB/s), both together 365 us, of which the scaling on its own would
+ * take 259: the squares read the last NORM_KEPT_BYTES through loads that leave them in the 256 MiB
+ * memory-side cache, where the scaling finds them (all of it through such loads: squares 136 us,
+ * together 375; none: 122 and 387; the scaling from the end backwards: 375).
  */
 #ifndef MP_GRADIENT_NORM_H
 #define MP_GRADIENT_NORM_H
@@ -27,10 +29,12 @@
 namespace mp {
 
 constexpr int NORM_RUNS = 120, NORM_THREADS = 256, NORM_PACKS = 4;
-constexpr size_t NORM_PIECE = (size_t)NORM_THREADS * NORM_PACKS * PACK_BYTES, NORM_PARTIALS = 2048;
+constexpr size_t NORM_PIECE = (size_t)NORM_THREADS * NORM_PACKS * PACK_BYTES, NORM_PARTIALS = 1024; /* a table */
 /* up to so many pieces the scaling adds up the partial sums itself, in every workgroup, and one launch is
  * saved; beyond, a workgroup would spend as long on that as on its piece */
 constexpr size_t NORM_FUSED_PIECES = 1024;
+
+constexpr size_t NORM_KEPT_BYTES = (size_t)224 << 20, NORM_KEPT_PIECES = NORM_KEPT_BYTES / NORM_PIECE;
 
 template <class T> struct NormTable {
   const T* src[NORM_RUNS];
@@ -40,16 +44,20 @@ template <class T> struct NormTable {
   int count;
 };
 
-/* The run that piece `q` belongs to: the last one whose first piece is not behind it. Runs have a piece at
- * least. Every lane looks at two of the first pieces, so the search is one load and a vote. */
+/* The run that piece `q` belongs to: the last one whose first piece is not behind it (runs have a piece at
+ * least). Scalar loads from the argument block; one vector load a wavefront and a vote cost the scaling
+ * of 100 runs 3 %. */
 template <class T> __device__ __forceinline__ int norm_run_of(const NormTable<T>& t, unsigned q) {
-  static_assert(NORM_RUNS <= 2 * WAVE, "two runs a lane");
-  const int lane = threadIdx.x % WAVE;
-  const bool lo = lane < t.count && t.first[lane] <= q, hi = lane + WAVE < t.count && t.first[lane + WAVE < NORM_RUNS ? lane + WAVE : 0] <= q;
-  return __popcll(__ballot(lo)) + __popcll(__ballot(hi)) - 1;
+  int lo = 0, hi = t.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (t.first[mid] <= q) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
 }
 
-/* A piece's packs in registers: f(pack index u, offset, elements that exist). */
+/* Where a piece lies: pack u of a thread is at(u) elements behind the piece's first. */
 template <class T> struct NormPiece {
   static constexpr int W = PACK_BYTES / (int)sizeof(T);
   static constexpr size_t LEN = NORM_PIECE / sizeof(T);
@@ -75,26 +83,37 @@ __device__ __forceinline__ double norm_block_sum(double s, double* slots) {
   return t;
 }
 
-template <class T> __global__ __launch_bounds__(NORM_THREADS) void gradient_squares(NormTable<T> t, double* partials) {
+template <bool KEEP, class T> __device__ __forceinline__ double piece_squares(const NormTable<T>& t, unsigned q) {
   constexpr int W = NormPiece<T>::W;
   using VL = typename loose_vec_of<T, W>::type;
-  __shared__ double slots[NORM_THREADS / WAVE];
+  const NormPiece<T> piece(t, q);
+  const T* src = t.src[piece.run] + piece.lo;
   double s = 0.0;
-  for (unsigned q = blockIdx.x; q < t.first[t.count]; q += gridDim.x) {
-    const NormPiece<T> piece(t, q);
-    const T* src = t.src[piece.run] + piece.lo;
-    if (piece.whole()) {
-      typename vec_of<T, W>::type v[NORM_PACKS];
+  if (piece.whole()) {
+    typename vec_of<T, W>::type v[NORM_PACKS];
 #pragma unroll
-      for (int u = 0; u < NORM_PACKS; ++u) v[u] = *reinterpret_cast<const VL*>(src + piece.at(u));
-#pragma unroll
-      for (int u = 0; u < NORM_PACKS; ++u)
-#pragma unroll
-        for (int j = 0; j < W; ++j) s += (double)v[u][j] * (double)v[u][j];
-    } else {
-      for (size_t i = threadIdx.x; i < piece.left; i += NORM_THREADS) s += (double)src[i] * (double)src[i];
+    for (int u = 0; u < NORM_PACKS; ++u) {
+      const VL* at = reinterpret_cast<const VL*>(src + piece.at(u));
+      v[u] = KEEP ? *at : __builtin_nontemporal_load(at);
     }
+#pragma unroll
+    for (int u = 0; u < NORM_PACKS; ++u)
+#pragma unroll
+      for (int j = 0; j < W; ++j) s += (double)v[u][j] * (double)v[u][j];
+  } else {
+    for (size_t i = threadIdx.x; i < piece.left; i += NORM_THREADS) s += (double)src[i] * (double)src[i];
   }
+  return s;
+}
+
+/* Pieces from `keep` on through loads that leave them in the memory-side cache. */
+template <class T> __global__ __launch_bounds__(NORM_THREADS) void gradient_squares(NormTable<T> t, unsigned keep, double* partials) {
+  __shared__ double slots[NORM_THREADS / WAVE];
+  const unsigned end = t.first[t.count];
+  double s = 0.0;
+  unsigned q = blockIdx.x;
+  for (; q < keep && q < end; q += gridDim.x) s += piece_squares<false>(t, q);
+  for (; q < end; q += gridDim.x) s += piece_squares<true>(t, q);
   s = norm_block_sum(s, slots);
   if (threadIdx.x == 0) partials[blockIdx.x] = s;
 }
@@ -121,7 +140,7 @@ __global__ __launch_bounds__(NORM_THREADS) void gradient_scaled(NormTable<T> t, 
   using P = typename precision<T>::type;
   constexpr int W = NormPiece<T>::W;
   using VL = typename loose_vec_of<T, W>::type;
-  const NormPiece<T> piece(t, t.first[t.count] - 1 - blockIdx.x); /* what was read last comes first */
+  const NormPiece<T> piece(t, blockIdx.x);
   const T* src = t.src[piece.run] + piece.lo;
   T* dst = t.dst[piece.run] + piece.lo;
   typename vec_of<T, W>::type v[NORM_PACKS];
@@ -205,14 +224,9 @@ inline void for_norm_tables(const void* const* grads, const void* const* outs, c
   if (t.count) f(t);
 }
 
-/* Partial sums a table of so many tensors may leave: all of them are added by one workgroup. Tensors that
- * form runs make fewer tables than they might, never more. */
-inline size_t norm_tables(size_t count) { return (count + NORM_RUNS - 1) / NORM_RUNS; }
-inline size_t norm_partials(size_t count) {
-  const size_t each = NORM_PARTIALS / (norm_tables(count) ? norm_tables(count) : 1);
-  return each < 64 ? 64 : each;
-}
-inline size_t gradient_norm_scratch_bytes(size_t count) { return norm_tables(count) * norm_partials(count) * sizeof(double); }
+/* Every table leaves at most NORM_PARTIALS sums. Tensors that form runs make fewer tables than they might,
+ * never more. */
+inline size_t gradient_norm_scratch_bytes(size_t count) { return (count + NORM_RUNS - 1) / NORM_RUNS * NORM_PARTIALS * sizeof(double); }
 
 /* Every argument, before the first launch. outs NULL where none are written. */
 template <class T>
@@ -245,10 +259,10 @@ inline void gradient_check_limit(const void* outs, double max_norm, size_t count
 template <class T>
 inline unsigned gradient_squares_all(const void* const* grads, const len_t* sizes, double* partials, size_t count, hipStream_t stream) {
   unsigned used = 0;
-  const unsigned cap = (unsigned)norm_partials(norm_work<T>(grads, nullptr, sizes, count).runs);
   for_norm_tables<T>(grads, nullptr, sizes, count, [&](const NormTable<T>& t) {
-    const unsigned pieces = t.first[t.count], blocks = pieces < cap ? pieces : cap;
-    gradient_squares<T><<<dim3(blocks), dim3(NORM_THREADS), 0, stream>>>(t, partials + used);
+    const unsigned pieces = t.first[t.count], blocks = pieces < NORM_PARTIALS ? pieces : (unsigned)NORM_PARTIALS;
+    const unsigned keep = pieces > NORM_KEPT_PIECES ? pieces - (unsigned)NORM_KEPT_PIECES : 0;
+    gradient_squares<T><<<dim3(blocks), dim3(NORM_THREADS), 0, stream>>>(t, keep, partials + used);
     MP_CHECK_LAUNCH();
     used += blocks;
   });
