@@ -11,7 +11,9 @@
  * then chunks of the sorted places are summed in registers, in precision<T>. An id whose places lie
  * within one chunk is written at once; one that crosses chunks leaves a partial row in each, and a
  * last kernel adds those in order. Rows of the table that no id names are cleared (or scaled, by
- * alpha) by workgroups of the same launch as the sums; with alpha = 1 they are not touched.
+ * alpha) by workgroups of the same launch as the sums; with alpha = 1 they are not touched. With
+ * alpha = 0 the sort's launches, which use a fraction of the GPU, clear the table's first rows on the
+ * way, named or not.
  */
 #ifndef MP_EMBEDDING_H
 #define MP_EMBEDDING_H
@@ -53,68 +55,64 @@ __global__ __launch_bounds__(256) void embedding_rows(
   rp.store(y + row * n, p, out);
 }
 
+/* ------------------------------------------------------------------ clearing rows */
+
+/* Rows [0, rows) of a table cleared by the workgroups of a launch from block `first` on, in units of
+ * FILL_PACKS packs a thread. */
+constexpr size_t FILL_PACKS = 4;
+template <class T, int THREADS> __device__ __forceinline__ void clear_part(T* table, size_t count, unsigned block) {
+  constexpr int W = PACK_BYTES / (int)sizeof(T);
+  using VL = typename loose_vec_of<T, W>::type;
+  const size_t lo = (size_t)block * (THREADS * FILL_PACKS * W);
+  typename vec_of<T, W>::type zero;
+#pragma unroll
+  for (int i = 0; i < W; ++i) zero[i] = (T)0;
+#pragma unroll
+  for (size_t u = 0; u < FILL_PACKS; ++u) {
+    const size_t i = lo + (u * THREADS + threadIdx.x) * W;
+    if (i + W <= count) __builtin_nontemporal_store(zero, reinterpret_cast<VL*>(table + i));
+    else
+      for (size_t j = i; j < count; ++j) table[j] = (T)0;
+  }
+}
+
 /* ------------------------------------------------------------------ sorting the places by id */
 
 /* A radix sort of 9 bits a pass, lowest first. A tile of the places belongs to one workgroup of 16
  * wavefronts, each of which takes an equal, contiguous part of it, so that counts alone say where
  * every place goes: the places of a digit in earlier tiles, in earlier wavefronts of the tile, and
- * earlier in the wavefront. Two launches a pass: count, then place (each workgroup of the second
- * adds up the counts of all tiles for itself). */
+ * earlier in the wavefront. Two launches a pass: count, then place (each workgroup of the second adds up
+ * the counts of all tiles for itself; counting the next pass's digits there with atomics saves a launch
+ * and loses more, because a common id's places all meet on one counter: 20 us a launch against 10 + 5).
+ * Up to SORT_SINGLE places are sorted by one workgroup in one launch. */
 constexpr int SORT_BITS = 9, SORT_DIGITS = 1 << SORT_BITS, SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / WAVE;
 constexpr size_t SORT_TILES = 256; /* tiles a pass, at most */
+constexpr int SORT_ROUNDS = 8;
+constexpr size_t SORT_SINGLE = (size_t)SORT_THREADS * SORT_ROUNDS;
 
 inline size_t sort_tile(size_t m) {
   const size_t each = (m + SORT_TILES - 1) / SORT_TILES;
   return (each + SORT_THREADS - 1) / SORT_THREADS * SORT_THREADS;
 }
+inline int sort_passes(size_t v) { /* keys run up to v */
+  int passes = 1;
+  while (v >> (passes * SORT_BITS)) ++passes;
+  return passes;
+}
 
 __device__ __forceinline__ unsigned sort_key(const void* tokens, unsigned wide, const unsigned* keys, size_t i, unsigned v) {
   return keys ? keys[i] : token_key(tokens, wide != 0, i, v);
 }
+__device__ __forceinline__ unsigned sort_digit(unsigned key, int shift) { return (key >> shift) & (SORT_DIGITS - 1); }
 
-static __global__ __launch_bounds__(SORT_THREADS) void embedding_sort_count(
-    const void* tokens, unsigned wide, const unsigned* keys, unsigned* counts, unsigned v, size_t m, size_t tile, int shift) {
-  __shared__ unsigned hist[SORT_DIGITS];
-  for (int d = threadIdx.x; d < SORT_DIGITS; d += SORT_THREADS) hist[d] = 0;
-  __syncthreads();
-  const size_t lo = (size_t)blockIdx.x * tile, hi = lo + tile < m ? lo + tile : m;
-  for (size_t i = lo + threadIdx.x; i < hi; i += SORT_THREADS)
-    atomicAdd(&hist[(sort_key(tokens, wide, keys, i, v) >> shift) & (SORT_DIGITS - 1)], 1u);
-  __syncthreads();
-  for (int d = threadIdx.x; d < SORT_DIGITS; d += SORT_THREADS) counts[(size_t)blockIdx.x * SORT_DIGITS + d] = hist[d];
-}
-
-/* keys NULL: the first pass, from the tokens; the place of an entry is then its index */
-static __global__ __launch_bounds__(SORT_THREADS) void embedding_sort_place(
-    const void* tokens, unsigned wide, const unsigned* keys, const unsigned* places, const unsigned* counts,
-    unsigned* keys_out, unsigned* places_out, unsigned v, size_t m, size_t tile, unsigned tiles, int shift) {
-  __shared__ unsigned next[SORT_WAVES][SORT_DIGITS]; /* counts of a wavefront's part, then where its next entry goes */
-  __shared__ unsigned total[2][SORT_DIGITS], before[2][SORT_DIGITS], wave_total[SORT_DIGITS / WAVE];
+/* Counts of the 512 digits by wavefront, turned into where each wavefront's first entry of a digit goes:
+ * every digit's start (the sums of the digits before it, and `before` of the thread's own digit) and then
+ * the wavefronts in turn. total: of the thread's digit, over everything that is sorted. Threads 0 to 511
+ * hold a digit each; all threads call it. */
+__device__ __forceinline__ void sort_starts(unsigned (*next)[SORT_DIGITS], unsigned* wave_total, unsigned total, unsigned before) {
   const int tid = threadIdx.x, wave = tid / WAVE, lane = tid % WAVE;
-  const size_t part = tile / SORT_WAVES, lo = (size_t)blockIdx.x * tile + wave * part;
-  const size_t hi = lo + part < m ? lo + part : m;
-
-  for (int d = lane; d < SORT_DIGITS; d += WAVE) next[wave][d] = 0;
-  __syncthreads();
-  for (size_t i = lo + lane; i < hi; i += WAVE)
-    atomicAdd(&next[wave][(sort_key(tokens, wide, keys, i, v) >> shift) & (SORT_DIGITS - 1)], 1u);
-
-  { /* two threads a digit add up the tiles */
-    const int d = tid & (SORT_DIGITS - 1), half = tid / SORT_DIGITS;
-    unsigned all = 0, mine = 0;
-    for (unsigned t = half; t < tiles; t += 2) {
-      const unsigned c = counts[(size_t)t * SORT_DIGITS + d];
-      all += c;
-      mine += t < blockIdx.x ? c : 0;
-    }
-    total[half][d] = all;
-    before[half][d] = mine;
-  }
-  __syncthreads();
-  unsigned sum = 0, inclusive = 0;
-  if (tid < SORT_DIGITS) { /* the digits' exclusive sums: within a wavefront, then over the eight */
-    sum = total[0][tid] + total[1][tid];
-    inclusive = sum;
+  unsigned inclusive = total;
+  if (tid < SORT_DIGITS) {
 #pragma unroll
     for (int step = 1; step < WAVE; step <<= 1) {
       const unsigned up = __shfl_up(inclusive, step, WAVE);
@@ -124,8 +122,9 @@ static __global__ __launch_bounds__(SORT_THREADS) void embedding_sort_place(
   }
   __syncthreads();
   if (tid < SORT_DIGITS) {
-    unsigned at = inclusive - sum + before[0][tid] + before[1][tid];
+    unsigned at = inclusive - total + before;
     for (int w = 0; w < wave; ++w) at += wave_total[w];
+#pragma unroll
     for (int w = 0; w < SORT_WAVES; ++w) {
       const unsigned c = next[w][tid];
       next[w][tid] = at;
@@ -133,27 +132,158 @@ static __global__ __launch_bounds__(SORT_THREADS) void embedding_sort_place(
     }
   }
   __syncthreads();
+}
+
+/* Where the 64 entries of a wavefront go, in order: behind those of the same digit in lower lanes, which
+ * votes on the digit's bits find. `starts` is the wavefront's row of `next`. */
+__device__ __forceinline__ unsigned sort_target(unsigned* starts, unsigned digit, bool live) {
+  const int lane = threadIdx.x % WAVE;
+  unsigned long long same = __ballot(live); /* the lanes that hold my digit */
+#pragma unroll
+  for (int b = 0; b < SORT_BITS; ++b) {
+    const bool set = (digit >> b) & 1u;
+    const unsigned long long with = __ballot(set);
+    same &= set ? with : ~with;
+  }
+  const unsigned earlier = (unsigned)__popcll(same & ((1ull << lane) - 1ull));
+  const unsigned at = (live ? starts[digit] : 0u) + earlier;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); /* every lane has read before the last of a digit moves it on */
+  if (live && (same >> lane) == 1ull) starts[digit] = at + 1u;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  return at;
+}
+
+/* Up to SORT_SINGLE places by workgroup 0; the others clear the table's first `cleared` elements. crossing:
+ * the counter of the ids that cross chunks, for the launches that follow. */
+template <class T>
+__global__ __launch_bounds__(SORT_THREADS) void embedding_sort_single(
+    const void* tokens, unsigned wide, unsigned* keys_out, unsigned* places_out, unsigned* crossing, unsigned v, unsigned m, int passes, T* table,
+    size_t cleared) {
+  if (blockIdx.x > 0) {
+    clear_part<T, SORT_THREADS>(table, cleared, blockIdx.x - 1);
+    return;
+  }
+  __shared__ unsigned next[SORT_WAVES][SORT_DIGITS], wave_total[SORT_DIGITS / WAVE];
+  __shared__ unsigned held_keys[SORT_SINGLE], held_places[SORT_SINGLE];
+  const int tid = threadIdx.x, wave = tid / WAVE, lane = tid % WAVE;
+  const unsigned rounds = (m + SORT_THREADS - 1) / SORT_THREADS, lo = wave * rounds * WAVE; /* of 64 entries, the wavefront's */
+  if (tid == 0) *crossing = 0;
+  unsigned key[SORT_ROUNDS], place[SORT_ROUNDS];
+#pragma unroll
+  for (int r = 0; r < SORT_ROUNDS; ++r) {
+    place[r] = lo + r * WAVE + lane;
+    key[r] = (unsigned)r < rounds && place[r] < m ? token_key(tokens, wide != 0, place[r], v) : 0u;
+  }
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * SORT_BITS;
+    for (int d = lane; d < SORT_DIGITS; d += WAVE) next[wave][d] = 0;
+    __syncthreads(); /* and what the pass before placed has been read */
+#pragma unroll
+    for (int r = 0; r < SORT_ROUNDS; ++r)
+      if ((unsigned)r < rounds && lo + r * WAVE + lane < m) atomicAdd(&next[wave][sort_digit(key[r], shift)], 1u);
+    __syncthreads();
+    unsigned total = 0;
+    if (tid < SORT_DIGITS)
+#pragma unroll
+      for (int w = 0; w < SORT_WAVES; ++w) total += next[w][tid];
+    sort_starts(next, wave_total, total, 0);
+    const bool last = pass == passes - 1;
+#pragma unroll
+    for (int r = 0; r < SORT_ROUNDS; ++r) {
+      if ((unsigned)r >= rounds) break;
+      const bool live = lo + r * WAVE + lane < m;
+      const unsigned at = sort_target(next[wave], sort_digit(key[r], shift), live);
+      if (live) {
+        held_keys[at] = key[r];
+        held_places[at] = place[r];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < SORT_ROUNDS; ++r) {
+      const unsigned i = lo + r * WAVE + lane;
+      if ((unsigned)r < rounds && i < m) {
+        key[r] = held_keys[i];
+        place[r] = held_places[i];
+        if (last) { /* in order: scattered to global memory by one workgroup they take longer than the sort */
+          keys_out[i] = key[r];
+          places_out[i] = place[r];
+        }
+      }
+    }
+  }
+}
+
+/* A pass's counts by tile. Workgroups from `tiles` on clear the table's first `cleared` elements. */
+template <class T>
+__global__ __launch_bounds__(SORT_THREADS) void embedding_sort_count(
+    const void* tokens, unsigned wide, const unsigned* keys, unsigned* counts, unsigned* crossing, unsigned v, size_t m, size_t tile, unsigned tiles,
+    int shift, T* table, size_t cleared) {
+  if (blockIdx.x >= tiles) {
+    clear_part<T, SORT_THREADS>(table, cleared, blockIdx.x - tiles);
+    return;
+  }
+  __shared__ unsigned hist[SORT_DIGITS];
+  for (int d = threadIdx.x; d < SORT_DIGITS; d += SORT_THREADS) hist[d] = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *crossing = 0;
+  __syncthreads();
+  const size_t lo = (size_t)blockIdx.x * tile, hi = lo + tile < m ? lo + tile : m;
+  for (size_t i = lo + threadIdx.x; i < hi; i += SORT_THREADS) atomicAdd(&hist[sort_digit(sort_key(tokens, wide, keys, i, v), shift)], 1u);
+  __syncthreads();
+  for (int d = threadIdx.x; d < SORT_DIGITS; d += SORT_THREADS) counts[blockIdx.x * SORT_DIGITS + d] = hist[d];
+}
+
+/* keys NULL: the first pass, from the tokens; the place of an entry is then its index. counts: this pass's, by tile. */
+template <class T>
+__global__ __launch_bounds__(SORT_THREADS) void embedding_sort_place(
+    const void* tokens, unsigned wide, const unsigned* keys, const unsigned* places, const unsigned* counts,
+    unsigned* keys_out, unsigned* places_out, unsigned v, size_t m, unsigned tile, unsigned tiles, int shift, T* table, size_t cleared) {
+  if (blockIdx.x >= tiles) {
+    clear_part<T, SORT_THREADS>(table, cleared, blockIdx.x - tiles);
+    return;
+  }
+  __shared__ unsigned next[SORT_WAVES][SORT_DIGITS]; /* counts of a wavefront's part, then where its next entry goes */
+  __shared__ unsigned total[SORT_DIGITS], before[SORT_DIGITS], wave_total[SORT_DIGITS / WAVE];
+  const int tid = threadIdx.x, wave = tid / WAVE, lane = tid % WAVE;
+  const unsigned part = tile / SORT_WAVES;
+  const size_t lo = (size_t)blockIdx.x * tile + wave * part, hi = lo + part < m ? lo + part : m;
+
+  for (int d = lane; d < SORT_DIGITS; d += WAVE) next[wave][d] = 0;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); /* a wavefront's row is its own */
+  for (size_t i = lo + lane; i < hi; i += WAVE) atomicAdd(&next[wave][sort_digit(sort_key(tokens, wide, keys, i, v), shift)], 1u);
+
+  /* two threads a digit add up the tiles, eight loads on their way */
+  const int d = tid & (SORT_DIGITS - 1), half = tid / SORT_DIGITS;
+  unsigned all = 0, mine = 0;
+  for (unsigned t0 = half; t0 < tiles; t0 += 16) {
+    unsigned c[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const unsigned t = t0 + 2 * u;
+      c[u] = counts[(t < tiles ? t : 0) * SORT_DIGITS + d];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const unsigned t = t0 + 2 * u;
+      all += t < tiles ? c[u] : 0;
+      mine += t < blockIdx.x ? c[u] : 0;
+    }
+  }
+  if (half == 1) {
+    total[d] = all;
+    before[d] = mine;
+  }
+  __syncthreads();
+  sort_starts(next, wave_total, half == 0 ? all + total[d] : 0, half == 0 ? mine + before[d] : 0);
   for (size_t i0 = lo; i0 < hi; i0 += WAVE) { /* in order: 64 entries at a time */
     const size_t i = i0 + lane;
     const bool live = i < hi;
     const unsigned key = live ? sort_key(tokens, wide, keys, i, v) : 0u;
     const unsigned place = live ? (places ? places[i] : (unsigned)i) : 0u;
-    const unsigned digit = (key >> shift) & (SORT_DIGITS - 1);
-    unsigned long long same = __ballot(live); /* the lanes that hold my digit */
-#pragma unroll
-    for (int b = 0; b < SORT_BITS; ++b) {
-      const bool set = (digit >> b) & 1u;
-      const unsigned long long with = __ballot(set);
-      same &= set ? with : ~with;
-    }
-    const unsigned earlier = (unsigned)__popcll(same & ((1ull << lane) - 1ull));
-    const unsigned base = live ? next[wave][digit] : 0u;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); /* every lane has read before the last of a digit moves it on */
-    if (live && (same >> lane) == 1ull) next[wave][digit] = base + earlier + 1u;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const unsigned at = sort_target(next[wave], sort_digit(key, shift), live);
     if (live) {
-      keys_out[base + earlier] = key;
-      places_out[base + earlier] = place;
+      keys_out[at] = key;
+      places_out[at] = place;
     }
   }
 }
@@ -173,22 +303,48 @@ __device__ __forceinline__ size_t lower_bound(const unsigned* keys, size_t m, un
 
 constexpr int FILL_ROWS = 64; /* rows of the table a clearing workgroup looks after */
 
+/* The places of one id, a run of equal keys, around entry i, as far as `reach` entries before and behind it:
+ * [begin, end). */
+struct Run { size_t begin, end; };
+__device__ __forceinline__ Run run_around(const unsigned* keys, size_t m, size_t i, size_t reach) {
+  const unsigned key = keys[i];
+  size_t lo = i > reach ? i - reach : 0, hi = i; /* the first equal one lies in [lo, hi] */
+  while (lo < hi) {
+    const size_t mid = (lo + hi) / 2;
+    if (keys[mid] < key) lo = mid + 1;
+    else hi = mid;
+  }
+  Run r;
+  r.begin = lo;
+  lo = i + 1; /* the first greater one in [lo, hi] */
+  hi = i + reach < m ? i + reach : m;
+  while (lo < hi) {
+    const size_t mid = (lo + hi) / 2;
+    if (keys[mid] == key) lo = mid + 1;
+    else hi = mid;
+  }
+  r.end = lo;
+  return r;
+}
+
 /* Workgroups below sum_blocks: G lanes hold a strip of G packs of the columns and walk one chunk of
- * the sorted places, 256 / G chunks a workgroup. The others clear (BLEND: scale) the rows of the table
- * that no id names. partials: two rows of n for every chunk, the first for an id that begins in an
- * earlier chunk, the second for one that goes on in the next. */
+ * the sorted places, 256 / G chunks a workgroup. An id of no more places than a chunk belongs to the chunk
+ * it begins in, which goes past its end for it; only longer ones are cut where a chunk ends. The others clear (BLEND: scale) the rows of the table
+ * from `row_begin` on that no id names. partials: two rows of n for every chunk, the first for an id that
+ * begins in an earlier chunk, the second for one that goes on in the next; the chunks where such an id begins
+ * are listed, in any order. */
 template <class T, int W, int G, bool BLEND, bool LOOSE>
 __global__ __launch_bounds__(256) void embedding_sum(
     const unsigned* keys, const unsigned* places, const T* dy, T* grads, typename precision<T>::type* partials,
-    typename precision<T>::type scale, typename precision<T>::type alpha, unsigned v, size_t m, size_t n, size_t chunk,
-    unsigned strips, unsigned sum_blocks) {
+    unsigned* crossing, unsigned* list, typename precision<T>::type scale, typename precision<T>::type alpha, unsigned v, size_t m, size_t n,
+    size_t chunk, unsigned strips, unsigned sum_blocks, size_t row_begin) {
   using P = typename precision<T>::type;
   using V = typename vec_of<T, W>::type;
   const RowPacks<T, W, LOOSE> rp(n);
 
   if (blockIdx.x >= sum_blocks) {
     __shared__ unsigned named[FILL_ROWS];
-    const size_t row0 = (size_t)(blockIdx.x - sum_blocks) * FILL_ROWS;
+    const size_t row0 = row_begin + (size_t)(blockIdx.x - sum_blocks) * FILL_ROWS;
     const unsigned rows = (unsigned)(v - row0 < FILL_ROWS ? v - row0 : FILL_ROWS);
     if (threadIdx.x < FILL_ROWS) {
       const unsigned key = (unsigned)row0 + threadIdx.x;
@@ -222,24 +378,36 @@ __global__ __launch_bounds__(256) void embedding_sum(
   const int sub = threadIdx.x / G, lane = threadIdx.x % G;
   const size_t c = (size_t)(blockIdx.x / strips) * (256 / G) + sub;
   const int p = (int)(blockIdx.x % strips) * G + lane;
-  const size_t lo = c * chunk;
+  size_t lo = c * chunk;
   if (lo >= m || p >= rp.npk) return;
-  const size_t hi = lo + chunk < m ? lo + chunk : m;
+  size_t hi = lo + chunk < m ? lo + chunk : m;
+  bool begun = false, goes_on = false; /* the first id began, the last one goes on in another chunk */
+  if (hi < m && keys[hi - 1] == keys[hi]) {
+    const Run r = run_around(keys, m, hi, chunk + 1);
+    goes_on = r.end - r.begin > chunk;
+    if (!goes_on) hi = r.end;
+  }
+  if (lo > 0 && keys[lo - 1] == keys[lo]) {
+    const Run r = run_around(keys, m, lo, chunk + 1);
+    begun = r.end - r.begin > chunk;
+    if (!begun) lo = r.end;
+  }
+  if (lo >= hi) return;
 
   P acc[W];
   unsigned current = keys[lo];
-  bool begun = lo > 0 && keys[lo - 1] == current; /* the id's first place lies in an earlier chunk */
   auto clear = [&]() {
 #pragma unroll
     for (int i = 0; i < W; ++i) acc[i] = (P)0;
   };
-  auto leave = [&](bool goes_on) {
+  auto leave = [&](bool cut) {
     if (current >= v) return; /* padded places */
-    if (begun || goes_on) {
+    if (begun || cut) {
       P* at = partials + (c * 2 + (begun ? 0 : 1)) * n + (size_t)p * W;
 #pragma unroll
       for (int i = 0; i < W; ++i)
         if (i < rp.valid(p)) at[i] = acc[i];
+      if (!begun && p == 0) list[atomicAdd(crossing, 1u)] = (unsigned)c;
       return;
     }
     T* row = grads + (size_t)current * n;
@@ -277,38 +445,71 @@ __global__ __launch_bounds__(256) void embedding_sum(
       for (int i = 0; i < W; ++i) acc[i] += (P)row[u][i];
     }
   }
-  leave(hi < m && keys[hi] == current);
+  leave(goes_on);
 }
 
-/* The ids that cross chunks: the chunk where such an id begins adds up its partial rows in order (a
- * workgroup owns 16 columns of it; 16 slices take the rows in turn, then the slices are added). */
-template <class T, bool BLEND>
+/* The ids that cross chunks: the partial rows of each are added up in order, in fp64. Workgroups take (id,
+ * strip of JOIN_LANES * CW columns) in turn; the slices of a workgroup take the partial rows in turn, four
+ * on their way, and are then added. */
+constexpr int JOIN_LANES = 64, JOIN_SLICES = 256 / JOIN_LANES;
+template <class T, int CW, bool BLEND>
 __global__ __launch_bounds__(256) void embedding_join(
-    const unsigned* keys, const typename precision<T>::type* partials, T* grads, typename precision<T>::type scale,
-    typename precision<T>::type alpha, unsigned v, size_t m, size_t n, size_t chunk, unsigned strips) {
+    const unsigned* keys, const typename precision<T>::type* partials, const unsigned* crossing, const unsigned* list, T* grads,
+    typename precision<T>::type scale, typename precision<T>::type alpha, size_t m, size_t n, size_t chunk, unsigned strips) {
   using P = typename precision<T>::type;
-  constexpr int COLS = 64, SLICES = 256 / COLS;
-  __shared__ double part[SLICES][COLS];
-  const size_t c = blockIdx.x / strips, lo = c * chunk, hi = lo + chunk;
-  if (hi >= m) return;
-  const unsigned key = keys[hi - 1];
-  if (key >= v || keys[hi] != key) return;
-  if (keys[lo] == key && lo > 0 && keys[lo - 1] == key) return; /* it began earlier */
-  const size_t end = key + 1 == 0 ? m : lower_bound(keys, m, key + 1); /* behind its last place */
-  const size_t later = (end - hi + chunk - 1) / chunk;
-  const int col = threadIdx.x % COLS, slice = threadIdx.x / COLS;
-  const size_t j = (size_t)(blockIdx.x % strips) * COLS + col;
-  double s = 0.0;
-  if (j < n)
-    for (size_t k = slice; k <= later; k += SLICES) s += (double)partials[((c + k) * 2 + (k == 0 ? 1 : 0)) * n + j];
-  part[slice][col] = s;
-  __syncthreads();
-  if (slice == 0 && j < n) {
-    for (int k = 1; k < SLICES; ++k) s += part[k][col];
-    T* at = grads + (size_t)key * n + j;
-    double out = (double)scale * s;
-    if constexpr (BLEND) out += (double)alpha * (double)*at;
-    *at = (T)out;
+  constexpr int COLS = JOIN_LANES * CW;
+  __shared__ double part[JOIN_SLICES][COLS + 1];
+  __shared__ unsigned ends[256 / WAVE];
+  const unsigned work = *crossing * strips;
+  const int l = threadIdx.x % JOIN_LANES, slice = threadIdx.x / JOIN_LANES;
+  for (unsigned q = blockIdx.x; q < work; q += gridDim.x) {
+    const size_t c = list[q / strips];
+    const unsigned key = keys[(c + 1) * chunk - 1]; /* the id that goes on in the chunk behind */
+    /* the chunks behind c that begin with the id: 256 at a time */
+    size_t later = 0;
+    for (;;) {
+      const size_t at = (c + 1 + later + threadIdx.x) * chunk;
+      const unsigned long long same = __ballot(at < m && keys[at] == key);
+      if (threadIdx.x % WAVE == 0) ends[threadIdx.x / WAVE] = (unsigned)__builtin_popcountll(same); /* sorted: the first ones */
+      __syncthreads();
+      unsigned found = 0;
+#pragma unroll
+      for (int w = 0; w < 256 / WAVE; ++w) found += ends[w];
+      later += found;
+      __syncthreads();
+      if (found < 256) break;
+    }
+    const size_t j = (size_t)(q % strips) * COLS + l * CW;
+    double s[CW];
+#pragma unroll
+    for (int i = 0; i < CW; ++i) s[i] = 0.0;
+    if (j < n) { /* CW > 1: n is a multiple of it */
+      for (size_t k0 = slice; k0 <= later; k0 += 4 * JOIN_SLICES) {
+        P t[4][CW];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const size_t k = k0 + u * JOIN_SLICES <= later ? k0 + u * JOIN_SLICES : k0;
+          load_pack_nt<P, CW>(partials + ((c + k) * 2 + (k == 0 ? 1 : 0)) * n + j, t[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int i = 0; i < CW; ++i) s[i] += k0 + u * JOIN_SLICES <= later ? (double)t[u][i] : 0.0;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < CW; ++i) part[slice][l * CW + i] = s[i];
+    __syncthreads();
+    for (int col = threadIdx.x; col < COLS && (size_t)(q % strips) * COLS + col < n; col += 256) {
+      double t = 0.0;
+#pragma unroll
+      for (int k = 0; k < JOIN_SLICES; ++k) t += part[k][col];
+      T* at = grads + (size_t)key * n + (size_t)(q % strips) * COLS + col;
+      double out = (double)scale * t;
+      if constexpr (BLEND) out += (double)alpha * (double)*at;
+      *at = (T)out;
+    }
+    __syncthreads();
   }
 }
 
@@ -327,10 +528,15 @@ inline size_t embedding_chunk(size_t m) {
   return chunk;
 }
 
-/* Workspace of the reverse: two pairs of keys and places that the sort writes in turn, the counts of
- * its tiles, and two partial rows a chunk. Every part starts on a 256-byte boundary. */
+/* Bytes of the table that a launch of the sort clears beside it: what the rest of the GPU writes in the time
+ * the sort takes anyway. */
+constexpr size_t SORT_SINGLE_CLEARS = (size_t)64 << 20, SORT_COUNT_CLEARS = (size_t)24 << 20, SORT_PLACE_CLEARS = (size_t)48 << 20;
+
+/* Workspace of the reverse: two pairs of keys and places that the sort writes in turn, the counts of its
+ * tiles, the ids that cross chunks with their number, and two partial rows a chunk. Every
+ * part starts on a 256-byte boundary. */
 struct EmbeddingScratch {
-  size_t keys[2], places[2], counts, partials, bytes;
+  size_t keys[2], places[2], counts, crossing, list, partials, bytes;
 };
 template <class T> inline EmbeddingScratch embedding_scratch(size_t m, size_t n) {
   EmbeddingScratch s{};
@@ -340,13 +546,16 @@ template <class T> inline EmbeddingScratch embedding_scratch(size_t m, size_t n)
     at += (bytes + 255) / 256 * 256;
     return here;
   };
-  for (int k = 0; k < 2; ++k) {
+  const size_t chunk = embedding_chunk(m), chunks = (m + chunk - 1) / chunk, pairs = m > SORT_SINGLE ? 2 : 1;
+  for (size_t k = 0; k < pairs; ++k) {
     s.keys[k] = take(m * sizeof(unsigned));
     s.places[k] = take(m * sizeof(unsigned));
   }
-  s.counts = take(SORT_TILES * SORT_DIGITS * sizeof(unsigned));
-  const size_t chunk = embedding_chunk(m);
-  s.partials = take((m + chunk - 1) / chunk * 2 * n * sizeof(typename precision<T>::type));
+  const size_t tile = sort_tile(m), tiles = m > SORT_SINGLE ? (m + tile - 1) / tile : 0;
+  s.counts = take(tiles * SORT_DIGITS * sizeof(unsigned));
+  s.crossing = take(sizeof(unsigned));
+  s.list = take(chunks * sizeof(unsigned));
+  s.partials = take(chunks * 2 * n * sizeof(typename precision<T>::type));
   s.bytes = at;
   return s;
 }
@@ -408,45 +617,80 @@ inline void embedding_reverse(const void* tokens, const T* dy, T* grads, void* s
   require(reinterpret_cast<uintptr_t>(scratch) % 16 == 0, "embedding reverse: scratch must be 16-byte aligned");
   const EmbeddingScratch at = embedding_scratch<T>(m, n);
   char* base = static_cast<char*>(scratch);
-  unsigned* keys[2] = {reinterpret_cast<unsigned*>(base + at.keys[0]), reinterpret_cast<unsigned*>(base + at.keys[1])};
-  unsigned* places[2] = {reinterpret_cast<unsigned*>(base + at.places[0]), reinterpret_cast<unsigned*>(base + at.places[1])};
-  unsigned* counts = reinterpret_cast<unsigned*>(base + at.counts);
+  auto words = [&](size_t offset) { return reinterpret_cast<unsigned*>(base + offset); };
+  unsigned *keys[2] = {words(at.keys[0]), words(at.keys[1])}, *places[2] = {words(at.places[0]), words(at.places[1])};
+  unsigned *counts = words(at.counts), *crossing = words(at.crossing), *list = words(at.list);
   P* partials = reinterpret_cast<P*>(base + at.partials);
 
-  const size_t tile = sort_tile(m);
-  const unsigned tiles = (unsigned)((m + tile - 1) / tile), wide = id_bytes == 8;
-  int from = -1; /* the tokens themselves */
-  for (int shift = 0; shift == 0 || (v >> shift) != 0; shift += SORT_BITS) { /* keys run up to v */
-    const unsigned *k = from < 0 ? nullptr : keys[from], *p = from < 0 ? nullptr : places[from];
-    const int to = from == 0 ? 1 : 0;
-    embedding_sort_count<<<dim3(tiles), dim3(SORT_THREADS), 0, stream>>>(tokens, wide, k, counts, (unsigned)v, m, tile, shift);
-    embedding_sort_place<<<dim3(tiles), dim3(SORT_THREADS), 0, stream>>>(tokens, wide, k, p, counts, keys[to], places[to], (unsigned)v, m,
-                                                                         tile, tiles, shift);
+  /* the sort, with a part of the clearing in each of its launches */
+  const unsigned wide = id_bytes == 8;
+  const int passes = sort_passes(v);
+  const size_t unit = (size_t)SORT_THREADS * FILL_PACKS * W; /* elements a clearing workgroup of a sort's launch takes */
+  const size_t elements = alpha == 0.0 ? v * n : 0;
+  size_t cleared = 0; /* elements so far, from the table's start */
+  auto share = [&](size_t bytes) { /* of the next launch: elements, a whole number of its workgroups' */
+    const size_t want = bytes / sizeof(T) / unit * unit, left = elements - cleared;
+    return want < left ? want : left;
+  };
+  const unsigned *sorted_keys, *sorted_places;
+  if (m <= SORT_SINGLE) {
+    const size_t part = share(SORT_SINGLE_CLEARS);
+    embedding_sort_single<T><<<dim3(1 + (unsigned)((part + unit - 1) / unit)), dim3(SORT_THREADS), 0, stream>>>(
+        tokens, wide, keys[0], places[0], crossing, (unsigned)v, (unsigned)m, passes, grads, part);
     MP_CHECK_LAUNCH();
-    from = to;
+    cleared += part;
+    sorted_keys = keys[0];
+    sorted_places = places[0];
+  } else {
+    const size_t tile = sort_tile(m);
+    const unsigned tiles = (unsigned)((m + tile - 1) / tile);
+    for (int pass = 0; pass < passes; ++pass) {
+      const int to = pass & 1;
+      const unsigned* from_keys = pass ? keys[to ^ 1] : nullptr;
+      size_t part = share(SORT_COUNT_CLEARS);
+      embedding_sort_count<T><<<dim3(tiles + (unsigned)((part + unit - 1) / unit)), dim3(SORT_THREADS), 0, stream>>>(
+          tokens, wide, from_keys, counts, crossing, (unsigned)v, m, tile, tiles, pass * SORT_BITS, grads + cleared, part);
+      MP_CHECK_LAUNCH();
+      cleared += part;
+      part = share(SORT_PLACE_CLEARS);
+      embedding_sort_place<T><<<dim3(tiles + (unsigned)((part + unit - 1) / unit)), dim3(SORT_THREADS), 0, stream>>>(
+          tokens, wide, from_keys, pass ? places[to ^ 1] : nullptr, counts, keys[to], places[to], (unsigned)v, m, (unsigned)tile, tiles,
+          pass * SORT_BITS, grads + cleared, part);
+      MP_CHECK_LAUNCH();
+      cleared += part;
+    }
+    sorted_keys = keys[(passes - 1) & 1];
+    sorted_places = places[(passes - 1) & 1];
   }
 
   const bool loose = !(aligned16(dy) && aligned16(grads) && n % W == 0);
   const size_t packs = (n + W - 1) / W, chunk = embedding_chunk(m), chunks = (m + chunk - 1) / chunk;
-  const size_t fill = alpha == 1.0 ? 0 : (v + FILL_ROWS - 1) / FILL_ROWS;
+  const size_t row_begin = cleared / n; /* rows from here on are still to be looked at, the first of them perhaps half cleared */
+  const size_t fill = alpha == 1.0 ? 0 : (v - row_begin + FILL_ROWS - 1) / FILL_ROWS;
   for_strip(packs, [&]<int G>() {
     const size_t strips = (packs + G - 1) / G, sums = (chunks + 256 / G - 1) / (256 / G) * strips;
     require(sums + fill < 0x7fffffffull, "embedding reverse: too many rows for one grid");
     const dim3 grid((unsigned)(sums + fill)), block(256);
     auto go = [&]<bool BLEND, bool LOOSE>() {
-      embedding_sum<T, W, G, BLEND, LOOSE><<<grid, block, 0, stream>>>(keys[from], places[from], dy, grads, partials, (P)scale, (P)alpha,
-                                                                       (unsigned)v, m, n, chunk, (unsigned)strips, (unsigned)sums);
+      embedding_sum<T, W, G, BLEND, LOOSE><<<grid, block, 0, stream>>>(sorted_keys, sorted_places, dy, grads, partials, crossing, list, (P)scale, (P)alpha,
+                                                                       (unsigned)v, m, n, chunk, (unsigned)strips, (unsigned)sums, row_begin);
     };
     if (alpha != 0.0) { if (loose) go.template operator()<true, true>(); else go.template operator()<true, false>(); }
     else { if (loose) go.template operator()<false, true>(); else go.template operator()<false, false>(); }
   });
   MP_CHECK_LAUNCH();
   if (chunks > 1) {
-    const size_t strips = (n + 63) / 64;
+    /* four columns a thread where the partial rows are 16-byte aligned */
+    constexpr bool FP32 = sizeof(P) == 4;
+    const bool four = FP32 && n % 4 == 0;
+    const size_t cols = JOIN_LANES * (four ? 4 : 1), strips = (n + cols - 1) / cols, cap = (size_t)compute_units() * 8;
     require(chunks * strips < 0x7fffffffull, "embedding reverse: too many rows for one grid");
-    const dim3 grid((unsigned)(chunks * strips)), block(256);
-    if (alpha != 0.0) embedding_join<T, true><<<grid, block, 0, stream>>>(keys[from], partials, grads, (P)scale, (P)alpha, (unsigned)v, m, n, chunk, (unsigned)strips);
-    else embedding_join<T, false><<<grid, block, 0, stream>>>(keys[from], partials, grads, (P)scale, (P)alpha, (unsigned)v, m, n, chunk, (unsigned)strips);
+    const dim3 grid((unsigned)((chunks - 1) * strips < cap ? (chunks - 1) * strips : cap)), block(256);
+    auto go = [&]<int CW, bool BLEND>() {
+      embedding_join<T, CW, BLEND><<<grid, block, 0, stream>>>(sorted_keys, partials, crossing, list, grads, (P)scale, (P)alpha, m, n, chunk, (unsigned)strips);
+    };
+    if (four) { if constexpr (FP32) { if (alpha != 0.0) go.template operator()<4, true>(); else go.template operator()<4, false>(); } }
+    else { if (alpha != 0.0) go.template operator()<1, true>(); else go.template operator()<1, false>(); }
     MP_CHECK_LAUNCH();
   }
 }
