@@ -83,12 +83,9 @@ template <class T, int THREADS> __device__ __forceinline__ void clear_part(T* ta
  * every place goes: the places of a digit in earlier tiles, in earlier wavefronts of the tile, and
  * earlier in the wavefront. Two launches a pass: count, then place (each workgroup of the second adds up
  * the counts of all tiles for itself; counting the next pass's digits there with atomics saves a launch
- * and loses more, because a common id's places all meet on one counter: 20 us a launch against 10 + 5).
- * Up to SORT_SINGLE places are sorted by one workgroup in one launch. */
+ * and loses more, because a common id's places all meet on one counter: 20 us a launch against 10 + 5). */
 constexpr int SORT_BITS = 9, SORT_DIGITS = 1 << SORT_BITS, SORT_THREADS = 1024, SORT_WAVES = SORT_THREADS / WAVE;
 constexpr size_t SORT_TILES = 256; /* tiles a pass, at most */
-constexpr int SORT_ROUNDS = 8;
-constexpr size_t SORT_SINGLE = (size_t)SORT_THREADS * SORT_ROUNDS;
 
 inline size_t sort_tile(size_t m) {
   const size_t each = (m + SORT_TILES - 1) / SORT_TILES;
@@ -153,64 +150,50 @@ __device__ __forceinline__ unsigned sort_target(unsigned* starts, unsigned digit
   return at;
 }
 
-/* Up to SORT_SINGLE places by workgroup 0; the others clear the table's first `cleared` elements. crossing:
- * the counter of the ids that cross chunks, for the launches that follow. */
+/* Up to RANK_MOST places without a radix sort: an entry goes behind the entries of smaller keys and the
+ * earlier ones of its own, so its place in the order is counted directly. A workgroup counts for 32 entries;
+ * the 32 half wavefronts of it take a share of all keys each, out of LDS, four to a broadcast read. Two
+ * instructions a pair of entries: for 8192 of them a tenth of what one workgroup's radix sort in LDS takes
+ * on its own CU (24 us). Workgroups from `groups` on clear the table's first `cleared` elements. */
+constexpr size_t RANK_MOST = 8192;
+constexpr int RANK_ENTRIES = 32, RANK_SHARES = SORT_THREADS / RANK_ENTRIES;
 template <class T>
-__global__ __launch_bounds__(SORT_THREADS) void embedding_sort_single(
-    const void* tokens, unsigned wide, unsigned* keys_out, unsigned* places_out, unsigned* crossing, unsigned v, unsigned m, int passes, T* table,
+__global__ __launch_bounds__(SORT_THREADS) void embedding_rank(
+    const void* tokens, unsigned wide, unsigned* keys_out, unsigned* places_out, unsigned* crossing, unsigned v, unsigned m, unsigned groups, T* table,
     size_t cleared) {
-  if (blockIdx.x > 0) {
-    clear_part<T, SORT_THREADS>(table, cleared, blockIdx.x - 1);
+  if (blockIdx.x >= groups) {
+    clear_part<T, SORT_THREADS>(table, cleared, blockIdx.x - groups);
     return;
   }
-  __shared__ unsigned next[SORT_WAVES][SORT_DIGITS], wave_total[SORT_DIGITS / WAVE];
-  __shared__ unsigned held_keys[SORT_SINGLE], held_places[SORT_SINGLE];
-  const int tid = threadIdx.x, wave = tid / WAVE, lane = tid % WAVE;
-  const unsigned rounds = (m + SORT_THREADS - 1) / SORT_THREADS, lo = wave * rounds * WAVE; /* of 64 entries, the wavefront's */
-  if (tid == 0) *crossing = 0;
-  unsigned key[SORT_ROUNDS], place[SORT_ROUNDS];
+  typedef unsigned uint4_t __attribute__((ext_vector_type(4)));
+  extern __shared__ unsigned rank_keys[]; /* m rounded up to a whole number of groups, the rest greater than any key */
+  __shared__ unsigned part[RANK_SHARES][RANK_ENTRIES];
+  const int tid = threadIdx.x, share = tid / RANK_ENTRIES, lane = tid % RANK_ENTRIES;
+  for (unsigned i = tid; i < groups * RANK_ENTRIES; i += SORT_THREADS) rank_keys[i] = i < m ? token_key(tokens, wide != 0, i, v) : 0xffffffffu;
+  if (blockIdx.x == 0 && tid == 0) *crossing = 0;
+  __syncthreads();
+  const unsigned mine = blockIdx.x, i = mine * RANK_ENTRIES + lane, key = rank_keys[i];
+  unsigned rank = 0;
+  for (unsigned b = share; b < groups; b += RANK_SHARES) {
+    const uint4_t* others = reinterpret_cast<const uint4_t*>(rank_keys + b * RANK_ENTRIES);
+    /* keys below `key`, or up to it in earlier groups: below key + 1 (no key is the largest number) */
+    const unsigned below = b < mine ? key + 1u : key;
 #pragma unroll
-  for (int r = 0; r < SORT_ROUNDS; ++r) {
-    place[r] = lo + r * WAVE + lane;
-    key[r] = (unsigned)r < rounds && place[r] < m ? token_key(tokens, wide != 0, place[r], v) : 0u;
+    for (int q = 0; q < RANK_ENTRIES / 4; ++q) {
+      const uint4_t o = others[q];
+      rank += (o[0] < below) + (o[1] < below) + (o[2] < below) + (o[3] < below);
+    }
+    if (b == mine)
+      for (int j = 0; j < RANK_ENTRIES; ++j) rank += rank_keys[b * RANK_ENTRIES + j] == key && j < lane;
   }
-  for (int pass = 0; pass < passes; ++pass) {
-    const int shift = pass * SORT_BITS;
-    for (int d = lane; d < SORT_DIGITS; d += WAVE) next[wave][d] = 0;
-    __syncthreads(); /* and what the pass before placed has been read */
+  part[share][lane] = rank;
+  __syncthreads();
+  if (tid < RANK_ENTRIES && i < m) {
+    unsigned at = 0;
 #pragma unroll
-    for (int r = 0; r < SORT_ROUNDS; ++r)
-      if ((unsigned)r < rounds && lo + r * WAVE + lane < m) atomicAdd(&next[wave][sort_digit(key[r], shift)], 1u);
-    __syncthreads();
-    unsigned total = 0;
-    if (tid < SORT_DIGITS)
-#pragma unroll
-      for (int w = 0; w < SORT_WAVES; ++w) total += next[w][tid];
-    sort_starts(next, wave_total, total, 0);
-    const bool last = pass == passes - 1;
-#pragma unroll
-    for (int r = 0; r < SORT_ROUNDS; ++r) {
-      if ((unsigned)r >= rounds) break;
-      const bool live = lo + r * WAVE + lane < m;
-      const unsigned at = sort_target(next[wave], sort_digit(key[r], shift), live);
-      if (live) {
-        held_keys[at] = key[r];
-        held_places[at] = place[r];
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < SORT_ROUNDS; ++r) {
-      const unsigned i = lo + r * WAVE + lane;
-      if ((unsigned)r < rounds && i < m) {
-        key[r] = held_keys[i];
-        place[r] = held_places[i];
-        if (last) { /* in order: scattered to global memory by one workgroup they take longer than the sort */
-          keys_out[i] = key[r];
-          places_out[i] = place[r];
-        }
-      }
-    }
+    for (int w = 0; w < RANK_SHARES; ++w) at += part[w][lane];
+    keys_out[at] = key;
+    places_out[at] = i;
   }
 }
 
@@ -301,7 +284,14 @@ __device__ __forceinline__ size_t lower_bound(const unsigned* keys, size_t m, un
   return lo;
 }
 
-constexpr int FILL_ROWS = 64; /* rows of the table a clearing workgroup looks after */
+/* Rows of the table that a workgroup of the sums' launch clears: about 16 KiB of them (r16 [65536] tokens of
+ * 151936 x 2048: 64 rows 204 us, 16 rows 186, 8 rows 180, 4 rows 176). */
+constexpr unsigned FILL_MOST = 64;
+constexpr size_t FILL_BYTES = 16384;
+inline unsigned embedding_fill_rows(size_t row_bytes) {
+  const size_t rows = FILL_BYTES / row_bytes;
+  return rows < 1 ? 1 : rows < FILL_MOST ? (unsigned)rows : FILL_MOST;
+}
 
 /* The places of one id, a run of equal keys, around entry i, as far as `reach` entries before and behind it:
  * [begin, end). */
@@ -337,39 +327,39 @@ template <class T, int W, int G, bool BLEND, bool LOOSE>
 __global__ __launch_bounds__(256) void embedding_sum(
     const unsigned* keys, const unsigned* places, const T* dy, T* grads, typename precision<T>::type* partials,
     unsigned* crossing, unsigned* list, typename precision<T>::type scale, typename precision<T>::type alpha, unsigned v, size_t m, size_t n,
-    size_t chunk, unsigned strips, unsigned sum_blocks, size_t row_begin) {
+    size_t chunk, unsigned strips, unsigned sum_blocks, size_t row_begin, unsigned fill_rows) {
   using P = typename precision<T>::type;
   using V = typename vec_of<T, W>::type;
   const RowPacks<T, W, LOOSE> rp(n);
 
   if (blockIdx.x >= sum_blocks) {
-    __shared__ unsigned named[FILL_ROWS];
-    const size_t row0 = row_begin + (size_t)(blockIdx.x - sum_blocks) * FILL_ROWS;
-    const unsigned rows = (unsigned)(v - row0 < FILL_ROWS ? v - row0 : FILL_ROWS);
-    if (threadIdx.x < FILL_ROWS) {
+    __shared__ unsigned named[FILL_MOST];
+    const size_t row0 = row_begin + (size_t)(blockIdx.x - sum_blocks) * fill_rows;
+    const unsigned rows = (unsigned)(v - row0 < fill_rows ? v - row0 : fill_rows);
+    if (threadIdx.x < rows) {
       const unsigned key = (unsigned)row0 + threadIdx.x;
-      unsigned there = 1;
-      if (threadIdx.x < rows) {
-        const size_t at = lower_bound(keys, m, key);
-        there = at < m && keys[at] == key;
-      }
-      named[threadIdx.x] = there;
+      const size_t at = lower_bound(keys, m, key);
+      named[threadIdx.x] = at < m && keys[at] == key;
     }
     __syncthreads();
-    for (unsigned k = 0; k < rows; ++k) {
-      if (named[k]) continue;
+    auto clear = [&](unsigned k, int p) {
+      if (named[k]) return;
       T* row = grads + (row0 + k) * n;
-      for (int p = threadIdx.x; p < rp.npk; p += 256) {
-        P out[W];
+      P out[W];
 #pragma unroll
-        for (int i = 0; i < W; ++i) out[i] = (P)0;
-        if constexpr (BLEND) {
-          rp.template load<true>(row, p, out);
+      for (int i = 0; i < W; ++i) out[i] = (P)0;
+      if constexpr (BLEND) {
+        rp.template load<true>(row, p, out);
 #pragma unroll
-          for (int i = 0; i < W; ++i) out[i] *= alpha;
-        }
-        rp.store(row, p, out);
+        for (int i = 0; i < W; ++i) out[i] *= alpha;
       }
+      rp.store(row, p, out);
+    };
+    if (rp.npk >= 256) {
+      for (unsigned k = 0; k < rows; ++k)
+        for (int p = threadIdx.x; p < rp.npk; p += 256) clear(k, p);
+    } else { /* several narrow rows at a time */
+      for (unsigned q = threadIdx.x; q < rows * (unsigned)rp.npk; q += 256) clear(q / (unsigned)rp.npk, (int)(q % (unsigned)rp.npk));
     }
     return;
   }
@@ -451,7 +441,7 @@ __global__ __launch_bounds__(256) void embedding_sum(
 /* The ids that cross chunks: the partial rows of each are added up in order, in fp64. Workgroups take (id,
  * strip of JOIN_LANES * CW columns) in turn; the slices of a workgroup take the partial rows in turn, four
  * on their way, and are then added. */
-constexpr int JOIN_LANES = 64, JOIN_SLICES = 256 / JOIN_LANES;
+constexpr int JOIN_LANES = 32, JOIN_SLICES = 256 / JOIN_LANES;
 template <class T, int CW, bool BLEND>
 __global__ __launch_bounds__(256) void embedding_join(
     const unsigned* keys, const typename precision<T>::type* partials, const unsigned* crossing, const unsigned* list, T* grads,
@@ -524,13 +514,13 @@ template <class T, bool BLEND> __global__ __launch_bounds__(256) void embedding_
 /* The sorted places one chunk holds. */
 inline size_t embedding_chunk(size_t m) {
   size_t chunk = 8;
-  while (chunk < 64 && m / chunk > 2048) chunk *= 2;
+  while (chunk < 32 && m / chunk > 1024) chunk *= 2;
   return chunk;
 }
 
 /* Bytes of the table that a launch of the sort clears beside it: what the rest of the GPU writes in the time
  * the sort takes anyway. */
-constexpr size_t SORT_SINGLE_CLEARS = (size_t)64 << 20, SORT_COUNT_CLEARS = (size_t)24 << 20, SORT_PLACE_CLEARS = (size_t)48 << 20;
+constexpr size_t RANK_CLEARS = (size_t)32 << 20, SORT_COUNT_CLEARS = (size_t)24 << 20, SORT_PLACE_CLEARS = (size_t)48 << 20;
 
 /* Workspace of the reverse: two pairs of keys and places that the sort writes in turn, the counts of its
  * tiles, the ids that cross chunks with their number, and two partial rows a chunk. Every
@@ -546,12 +536,12 @@ template <class T> inline EmbeddingScratch embedding_scratch(size_t m, size_t n)
     at += (bytes + 255) / 256 * 256;
     return here;
   };
-  const size_t chunk = embedding_chunk(m), chunks = (m + chunk - 1) / chunk, pairs = m > SORT_SINGLE ? 2 : 1;
+  const size_t chunk = embedding_chunk(m), chunks = (m + chunk - 1) / chunk, pairs = m > RANK_MOST ? 2 : 1;
   for (size_t k = 0; k < pairs; ++k) {
     s.keys[k] = take(m * sizeof(unsigned));
     s.places[k] = take(m * sizeof(unsigned));
   }
-  const size_t tile = sort_tile(m), tiles = m > SORT_SINGLE ? (m + tile - 1) / tile : 0;
+  const size_t tile = sort_tile(m), tiles = m > RANK_MOST ? (m + tile - 1) / tile : 0;
   s.counts = take(tiles * SORT_DIGITS * sizeof(unsigned));
   s.crossing = take(sizeof(unsigned));
   s.list = take(chunks * sizeof(unsigned));
@@ -633,10 +623,11 @@ inline void embedding_reverse(const void* tokens, const T* dy, T* grads, void* s
     return want < left ? want : left;
   };
   const unsigned *sorted_keys, *sorted_places;
-  if (m <= SORT_SINGLE) {
-    const size_t part = share(SORT_SINGLE_CLEARS);
-    embedding_sort_single<T><<<dim3(1 + (unsigned)((part + unit - 1) / unit)), dim3(SORT_THREADS), 0, stream>>>(
-        tokens, wide, keys[0], places[0], crossing, (unsigned)v, (unsigned)m, passes, grads, part);
+  if (m <= RANK_MOST) {
+    const size_t part = share(RANK_CLEARS);
+    const unsigned groups = (unsigned)((m + RANK_ENTRIES - 1) / RANK_ENTRIES);
+    embedding_rank<T><<<dim3(groups + (unsigned)((part + unit - 1) / unit)), dim3(SORT_THREADS), groups * RANK_ENTRIES * sizeof(unsigned), stream>>>(
+        tokens, wide, keys[0], places[0], crossing, (unsigned)v, (unsigned)m, groups, grads, part);
     MP_CHECK_LAUNCH();
     cleared += part;
     sorted_keys = keys[0];
@@ -666,14 +657,15 @@ inline void embedding_reverse(const void* tokens, const T* dy, T* grads, void* s
   const bool loose = !(aligned16(dy) && aligned16(grads) && n % W == 0);
   const size_t packs = (n + W - 1) / W, chunk = embedding_chunk(m), chunks = (m + chunk - 1) / chunk;
   const size_t row_begin = cleared / n; /* rows from here on are still to be looked at, the first of them perhaps half cleared */
-  const size_t fill = alpha == 1.0 ? 0 : (v - row_begin + FILL_ROWS - 1) / FILL_ROWS;
+  const unsigned fill_rows = embedding_fill_rows(n * sizeof(T));
+  const size_t fill = alpha == 1.0 ? 0 : (v - row_begin + fill_rows - 1) / fill_rows;
   for_strip(packs, [&]<int G>() {
     const size_t strips = (packs + G - 1) / G, sums = (chunks + 256 / G - 1) / (256 / G) * strips;
     require(sums + fill < 0x7fffffffull, "embedding reverse: too many rows for one grid");
     const dim3 grid((unsigned)(sums + fill)), block(256);
     auto go = [&]<bool BLEND, bool LOOSE>() {
       embedding_sum<T, W, G, BLEND, LOOSE><<<grid, block, 0, stream>>>(sorted_keys, sorted_places, dy, grads, partials, crossing, list, (P)scale, (P)alpha,
-                                                                       (unsigned)v, m, n, chunk, (unsigned)strips, (unsigned)sums, row_begin);
+                                                                       (unsigned)v, m, n, chunk, (unsigned)strips, (unsigned)sums, row_begin, fill_rows);
     };
     if (alpha != 0.0) { if (loose) go.template operator()<true, true>(); else go.template operator()<true, false>(); }
     else { if (loose) go.template operator()<false, true>(); else go.template operator()<false, false>(); }
