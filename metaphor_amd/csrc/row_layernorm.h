@@ -875,7 +875,9 @@ inline void layernorm_reverse(const T* x, const T* gain, const T* dy, T* dx, T* 
   if (n == 0) return;
   constexpr int W = PACK_BYTES / (int)sizeof(T);
   require(n <= 0x40000000ull, "layernorm reverse: row length must not exceed 2^30");
+  require(dg != db || dg == nullptr, "layernorm reverse: gain_grads and bias_grads must be different vectors");
   require(m == 0 || scratch != nullptr, "layernorm reverse: scratch must hold mpLayernormReverseScratchBytes bytes");
+  require(reinterpret_cast<uintptr_t>(scratch) % sizeof(typename precision<T>::type) == 0, "layernorm reverse: scratch must be aligned to its sums");
   layernorm_reverse_as<T>(layernorm_reverse_plan<T>((n + W - 1) / W), x, gain, dy, dx, dg, db, scratch, eps, alpha, m, n, stream);
 }
 

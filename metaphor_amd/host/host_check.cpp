@@ -328,6 +328,57 @@ static int row_ops(mp::Stream stream) {
   return 0;
 }
 
+/* A token model's step through the graph: embedding -> layer norm -> product -> softmax, the reverse from an
+ * upstream gradient, twice, and the weights' gradients clipped; dumped for the check against 64 bits. */
+static int token_model(mp::Stream stream) {
+  mp::Graph* G = mp::Graph::init({stream, mp::Mode::train});
+  const size_t v = 50, m = 37, n = 24, k = 11;
+  Rng r{29};
+  const auto ht = r.normal(v * n, 0, 1), hg = r.normal(n, 1, 0.1), hb = r.normal(n, 0, 0.1), hw = r.normal(n * k, 0, 0.3), hd = r.normal(m * k, 0, 1);
+  std::vector<int32_t> ids(m);
+  for (size_t i = 0; i < m; ++i) ids[i] = i % 9 == 4 ? -1 : (int32_t)(r.next() * r.next() * (double)v);
+  void* device_ids = mpMemAlloc(m * sizeof(int32_t), stream->context);
+  mpMemcpyHtoD(device_ids, ids.data(), m * sizeof(int32_t), stream->context);
+  mpStreamSynchronize(stream->context);
+  mp::Tensor table = leaf(G, mp::TensorClass::wgt, {v, n}, ht), g = leaf(G, mp::TensorClass::wgt, {n}, hg), b = leaf(G, mp::TensorClass::wgt, {n}, hb);
+  mp::Tensor w = leaf(G, mp::TensorClass::wgt, {n, k}, hw);
+  dump("tok_table", ht); dump("tok_gain", hg); dump("tok_bias", hb); dump("tok_w", hw); dump("tok_dp", hd); dump("tok_ids", ids);
+
+  mp::Tensor x = mp::ops::embedding(table, {device_ids, m, sizeof(int32_t)}, 2.0);
+  mp::Tensor h = mp::ops::layernorm(x, g, b, 1e-5);
+  mp::Tensor p = mp::ops::softmax(mp::ops::inner_product(h, w, "ij,jk->ik"));
+  dump("tok_x", x.native<float>()); dump("tok_h", h.native<float>()); dump("tok_p", p.native<float>());
+  set_grad(p, hd);
+  p.reverse(mp::ReverseCleanup::keep);
+  dump("tok_dtable", table.native_grad<float>()); dump("tok_dgain", g.native_grad<float>()); dump("tok_dbias", b.native_grad<float>());
+  dump("tok_dw", w.native_grad<float>());
+
+  /* the same again on top of it: every gradient doubles; no bias this time, on a second branch */
+  mp::Tensor x2 = mp::ops::embedding(table, {device_ids, m, sizeof(int32_t)}, 2.0);
+  mp::Tensor h2 = mp::ops::layernorm(x2, g, 1e-5);
+  set_grad(h2, h.native<float>());
+  h2.reverse(mp::ReverseCleanup::keep);
+  dump("tok_dtable2", table.native_grad<float>()); dump("tok_dgain2", g.native_grad<float>());
+
+  /* a weight of another dtype under the same norm */
+  mp::Tensor d = G->tensor(mp::TensorClass::wgt, mp::Tag::r64, {5});
+  mp::enable_gradient(d);
+  const std::vector<double> hdd = {3.0, -4.0, 0.5, 0.0, 1.0};
+  mpMemcpyHtoD(d.grad_ptr(), hdd.data(), 5 * sizeof(double), stream->context);
+  mpStreamSynchronize(stream->context);
+  G->clip_gradients(0.75);
+  dump("tok_norm", std::vector<double>{G->gradient_norm()});
+  dump("tok_clipped_table", table.native_grad<float>()); dump("tok_clipped_bias", b.native_grad<float>());
+  dump("tok_clipped_d", d.native_grad<double>());
+  mp::Graph* E = mp::Graph::init({stream, mp::Mode::eval});
+  E->clip_gradients(1.0); /* nothing to clip */
+  CHECK(E->gradient_norm() == 0.0);
+  E->deinit();
+  mpMemFree(device_ids, stream->context);
+  G->deinit();
+  return 0;
+}
+
 /* Part 3: the matrix side of the surface. First the reference's own example with its hand-computable
  * answers (src/examples/experimental.zig:19-62), then every inner-product expression, permutate,
  * reduce / broadcast, dilate and translate on random operands, dumped for the oracle check, and a
@@ -482,6 +533,8 @@ int main(int argc, char** argv) {
   printf("host_check: fused chain ok (one kernel forward, one kernel reverse)\n");
   if (row_ops(stream)) return 1;
   printf("host_check: softmax / rmsnorm through the graph ok\n");
+  if (token_model(stream)) return 1;
+  printf("host_check: embedding / layer norm / clipping through the graph ok\n");
   if (matrix_ops(stream)) return 1;
   printf("host_check: inner products, permutate, reduce / broadcast, checkpoint files ok\n");
 

@@ -116,6 +116,7 @@ void Graph::deinit() {
   reset(ResetGroup::node, ResetComponent::all);
   reset(ResetGroup::leaf, ResetComponent::all);
   allocator_.deinit(stream);
+  if (norm_) mpMemFree(norm_, stream->context);
   mpStreamSynchronize(stream->context);
   delete this;
 }
@@ -716,6 +717,40 @@ static double first_touch(Tensor t) {
   return 0.0;
 }
 
+/* args: x, gain, bias where there is one, eps, output */
+static void layernorm_reverse(const std::vector<OpDatum>& a) {
+  const bool biased = a.size() == 5;
+  const Tensor x = a[0].t, gain = a[1].t, z = a.back().t;
+  const double eps = a[a.size() - 2].s;
+  bool fresh = true;
+  const size_t operands = biased ? 3 : 2;
+  for (size_t i = 0; i < operands; ++i) fresh = fresh && !a[i].t.has_grad();
+  for (size_t i = 0; i < operands; ++i) {
+    const Tensor t = a[i].t;
+    if (fresh) t.ptr->grad_of(t) = t.ptr->allocator_.alloc(t.dtype(), t.len(), t.ptr->stream);
+    else enable_gradient(t);
+  }
+  const size_t n = z.sizes().back(), m = z.len() / n;
+  void* scratch = z.stream()->get_scratch(mpLayernormReverseScratchBytes((len_t)dkey(z), (len_t)m, (len_t)n));
+  kernels::layernorm_ij_j_reverse(dkey(z), x.data_ptr(), gain.data_ptr(), z.grad_ptr(), x.grad_ptr(), gain.grad_ptr(),
+                                  biased ? a[2].t.grad_ptr() : nullptr, scratch, eps, fresh ? 0.0 : 1.0, (len_t)m, (len_t)n,
+                                  z.context());
+  z.ptr->launches += 2;
+}
+
+/* args: table, tokens, scale, output. The launcher enqueues as many kernels as the number of tokens asks
+ * for; it counts as one. */
+static void embedding_reverse(const std::vector<OpDatum>& a) {
+  const Tensor table = a[0].t, z = a[3].t;
+  const Tokens ids = a[1].ids;
+  const double alpha = first_touch(table);
+  const len_t v = (len_t)table.sizes()[0], n = (len_t)table.sizes()[1], m = (len_t)ids.count;
+  void* scratch = z.stream()->get_scratch(mpEmbeddingReverseScratchBytes((len_t)dkey(z), v, m, n));
+  kernels::embedding_i_ij_reverse(dkey(z), ids.ptr, z.grad_ptr(), table.grad_ptr(), scratch, a[2].s, alpha, (len_t)ids.id_bytes, v, m, n,
+                                  z.context());
+  z.ptr->launches++;
+}
+
 /* column sums with the workspace that lets tall, narrow matrices use the whole GPU */
 static void column_sums(Graph* g, size_t key, const void* src, void* dst, double alpha, size_t m, size_t n) {
   const len_t bytes = mpReduceScratchBytes((len_t)key, (len_t)m, (len_t)n);
@@ -881,6 +916,43 @@ Tensor rmsnorm(Tensor x, Tensor gain, double eps) {
   return z;
 }
 
+static Tensor layernorm_of(Tensor x, Tensor gain, const Tensor* bias, double eps) {
+  if (x.dtype() != gain.dtype() || (bias && x.dtype() != bias->dtype())) panic("layernorm: x, gain and bias must agree in dtype");
+  if (x.same(gain) || (bias && (x.same(*bias) || gain.same(*bias)))) panic("layernorm: x, gain and bias must be different tensors");
+  if (gain.len() != x.sizes().back()) panic("layernorm: gain must have one entry per column");
+  if (bias && bias->len() != x.sizes().back()) panic("layernorm: bias must have one entry per column");
+  Graph* g = x.ptr;
+  void* px = x.data_ptr();
+  void* pg = gain.data_ptr();
+  void* pb = bias ? bias->data_ptr() : nullptr;
+  Tensor z = g->tensor(TensorClass::hid, x.dtype(), x.sizes());
+  const size_t n = x.sizes().back(), m = x.len() / n;
+  kernels::layernorm_ij_j(dkey(z), px, pg, pb, z.data_ptr(), eps, (len_t)m, (len_t)n, z.context());
+  g->launches++;
+  if (g->mode == Mode::train) {
+    if (bias) attach_op(z, layernorm_reverse, {x, gain, *bias, eps, z});
+    else attach_op(z, layernorm_reverse, {x, gain, eps, z});
+  }
+  return z;
+}
+Tensor layernorm(Tensor x, Tensor gain, Tensor bias, double eps) { return layernorm_of(x, gain, &bias, eps); }
+Tensor layernorm(Tensor x, Tensor gain, double eps) { return layernorm_of(x, gain, nullptr, eps); }
+
+Tensor embedding(Tensor table, Tokens tokens, double scale) {
+  if (table.rank() != 2) panic("embedding: the table must have rank 2");
+  if (tokens.count == 0 || !tokens.ptr) panic("embedding: there must be token ids");
+  if (tokens.id_bytes != 4 && tokens.id_bytes != 8) panic("embedding: token ids are 4 or 8 bytes wide");
+  Graph* g = table.ptr;
+  void* pt = table.data_ptr();
+  const size_t v = table.sizes()[0], n = table.sizes()[1];
+  Tensor z = g->tensor(TensorClass::hid, table.dtype(), {tokens.count, n});
+  kernels::embedding_i_ij(dkey(z), pt, tokens.ptr, z.data_ptr(), scale, (len_t)tokens.id_bytes, (len_t)v, (len_t)tokens.count, (len_t)n,
+                          z.context());
+  g->launches++;
+  if (g->mode == Mode::train) attach_op(z, embedding_reverse, {table, tokens, scale, z});
+  return z;
+}
+
 Tensor translate(Tensor x, double value) { return defer(x.ptr, Pending::translate, x, x, value); }
 
 Tensor dilate(Tensor x, double value) { return defer(x.ptr, Pending::dilate, x, x, value); }
@@ -1009,6 +1081,54 @@ void load_tensor(const std::string& dir, const std::string& filename, Tensor x) 
 }
 
 }  // namespace io
+
+void Graph::clip_gradients(double max_norm) {
+  if (!(max_norm >= 0.0)) panic("Graph.clip_gradients: the largest norm must not be negative");
+  if (!norm_) norm_ = mpMemAlloc(sizeof(double), stream->context);
+  if (!norm_) panic("Graph.clip_gradients: device allocation failed");
+  std::vector<void*> grads[3];
+  std::vector<len_t> sizes[3];
+  for (const Leaf& leaf : leaves_) {
+    if (leaf.cls != TensorClass::wgt || !leaf.grad.ptr) continue;
+    grads[(int)leaf.grad.dtype].push_back(leaf.grad.ptr);
+    sizes[(int)leaf.grad.dtype].push_back((len_t)leaf.grad.len);
+  }
+  size_t kinds = 0, only = 0, most = 0;
+  for (size_t key = 0; key < 3; ++key) {
+    if (grads[key].empty()) continue;
+    ++kinds;
+    only = key;
+    const size_t bytes = (size_t)mpGradientNormScratchBytes((len_t)key, (len_t)grads[key].size());
+    if (bytes > most) most = bytes;
+  }
+  void* scratch = most ? stream->get_scratch(most) : nullptr;
+  if (kinds <= 1) { /* one call; of no tensors, it leaves a norm of zero */
+    kernels::gradient_clip(only, grads[only].data(), grads[only].data(), sizes[only].data(), norm_, scratch, max_norm, (len_t)grads[only].size(),
+                           stream->context);
+    launches++;
+    return;
+  }
+  double alpha = 0.0;
+  for (size_t key = 0; key < 3; ++key) {
+    if (grads[key].empty()) continue;
+    kernels::gradient_norm(key, grads[key].data(), sizes[key].data(), norm_, scratch, alpha, (len_t)grads[key].size(), stream->context);
+    launches++;
+    alpha = 1.0;
+  }
+  for (size_t key = 0; key < 3; ++key) {
+    if (grads[key].empty()) continue;
+    kernels::gradient_scale(key, grads[key].data(), grads[key].data(), sizes[key].data(), norm_, max_norm, (len_t)grads[key].size(), stream->context);
+    launches++;
+  }
+}
+
+double Graph::gradient_norm() {
+  if (!norm_) panic("Graph.gradient_norm: no gradients have been clipped");
+  double value = 0.0;
+  mpMemcpyDtoH(&value, norm_, sizeof(double), stream->context);
+  mpStreamSynchronize(stream->context);
+  return value;
+}
 
 void Graph::save(const std::string& dir, const std::string& prefix) {
   size_t wgt_idx = 0;

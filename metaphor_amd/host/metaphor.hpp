@@ -9,7 +9,8 @@
  *   mp::Graph / mp::Tensor / GraphConfig / TensorClass  src/core/graph.zig:28-121, 256-363, 500-631
  *   mp::ops::{add, sub, hadamard, translate, dilate, relu, reduce, broadcast, inner_product,
  *             inner_product_scaled, permutate}           src/metaphor.zig:44-56, src/ops/*.zig
- *   mp::ops::{selu, softmax, rmsnorm}                   new ops in the same shape
+ *   mp::ops::{selu, softmax, rmsnorm, layernorm, embedding}   new ops in the same shape
+ *   Graph::clip_gradients                               the weights' gradients scaled to a largest norm
  *   mp::io::{save_tensor, load_tensor}, Graph::{save, load}   src/core/tensor_file.zig
  *   mp::algo::{fill, copy, sequence}, mp::util::{to_device, from_device}, mp::stream::Group<N>
  * Errors follow the reference: an impossible request panics (prints and aborts), nothing returns
@@ -136,12 +137,21 @@ struct Tensor {
   }
 };
 
-/* src/core/graph.zig:776-829: a tensor, a scalar or an index expression such as "ij,jk->ik" */
+/* Token ids: `count` signed integers of id_bytes (4 or 8) each on the device. They are borrowed, and must
+ * stay as they are until the reverse of every op they were given to has run. */
+struct Tokens {
+  const void* ptr = nullptr;
+  size_t count = 0, id_bytes = 8;
+};
+
+/* src/core/graph.zig:776-829: a tensor, a scalar or an index expression such as "ij,jk->ik"; token ids */
 struct OpDatum {
-  enum Kind { tensor, scalar, expr } kind = tensor;
+  enum Kind { tensor, scalar, expr, tokens } kind = tensor;
   Tensor t{};
   double s = 0.0;
   std::string e;
+  Tokens ids{};
+  OpDatum(Tokens x) : kind(tokens), ids(x) {}
   OpDatum(Tensor x) : kind(tensor), t(x) {}
   OpDatum(double v) : kind(scalar), s(v) {}
   OpDatum(const char* x) : kind(expr), e(x) {}
@@ -218,6 +228,12 @@ class Graph {
   void save(const std::string& dir, const std::string& prefix);
   void load(const std::string& dir, const std::string& prefix);
 
+  /* Every weight leaf's gradient times min(1, max_norm / norm), in place, with the norm of all of them
+   * together (whatever their dtypes). Nothing waits for the device; gradient_norm() does, and returns
+   * the norm the last call found. */
+  void clip_gradients(double max_norm);
+  double gradient_norm();
+
   /* core internals, public to the op modules as src/core/root.zig exports them */
   struct Leaf {
     TensorData data, grad;
@@ -236,6 +252,7 @@ class Graph {
   };
   std::vector<Leaf> leaves_;
   std::vector<Node> nodes_;
+  void* norm_ = nullptr; /* one double on the device */
   TensorAllocator allocator_;
 
   void reverse(size_t idx, ReverseCleanup cleanup);
@@ -274,6 +291,11 @@ Tensor inner_product_scaled(Tensor x, Tensor y, double scale, const char* expr);
 /* expr names the axis in the reference's notation; "ij|j" (rows over the last dim) is supported */
 Tensor softmax(Tensor x, const char* expr = "ij|j");
 Tensor rmsnorm(Tensor x, Tensor gain, double eps);
+/* (x - mean) / sqrt(var + eps) * gain (+ bias) over the last dimension */
+Tensor layernorm(Tensor x, Tensor gain, Tensor bias, double eps);
+Tensor layernorm(Tensor x, Tensor gain, double eps);
+/* row i = scale * table[tokens[i]], zeros for an id outside the table (a padded place) */
+Tensor embedding(Tensor table, Tokens tokens, double scale = 1.0);
 }  // namespace ops
 
 namespace algo {

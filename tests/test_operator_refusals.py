@@ -12,8 +12,10 @@ FAKE = 0x100000000000  # an address nothing dereferences: the call ends before a
 
 CASES = [
     ("layernorm_ij_j", f"{FAKE}, {FAKE}, {FAKE}, {FAKE}, 1e-5, 4, (1 << 30) + 1", "row length must not exceed"),
-    ("layernorm_ij_j_reverse", f"{FAKE}, {FAKE}, {FAKE}, {FAKE}, {FAKE}, {FAKE}, None, 1e-5, 0.0, 4, 64", "mpLayernormReverseScratchBytes"),
+    ("layernorm_ij_j_reverse", f"{FAKE}, {FAKE}, {FAKE}, {FAKE}, {FAKE}, {FAKE + 512}, None, 1e-5, 0.0, 4, 64", "mpLayernormReverseScratchBytes"),
     ("layernorm_ij_j_reverse", f"{FAKE}, {FAKE}, {FAKE}, {FAKE}, {FAKE}, {FAKE}, {FAKE}, 1e-5, 0.0, 4, (1 << 30) + 1", "row length must not exceed"),
+    ("layernorm_ij_j_reverse", f"{FAKE}, {FAKE}, {FAKE}, {FAKE}, {FAKE}, {FAKE}, {FAKE + 64}, 1e-5, 0.0, 4, 64", "must be different vectors"),
+    ("layernorm_ij_j_reverse", f"{FAKE}, {FAKE}, {FAKE}, {FAKE}, {FAKE}, {FAKE + 512}, {FAKE + 2}, 1e-5, 0.0, 4, 64", "aligned to its sums"),
     ("embedding_i_ij", f"{FAKE}, {FAKE}, {FAKE}, 1.0, 2, 10, 4, 64", "4 or 8 bytes wide"),
     ("embedding_i_ij", f"{FAKE}, {FAKE + 4}, {FAKE}, 1.0, 8, 10, 4, 64", "aligned to their width"),
     ("embedding_i_ij", f"{FAKE}, {FAKE}, {FAKE}, 1.0, 8, (1 << 32) - 1, 4, 64", "fewer than 2^32 - 1 rows"),
