@@ -6,9 +6,10 @@
  *   reverse   dT_kj = s * sum_{i: t_i = k} dy_ij + alpha * dT_kj
  * An id outside [0, v) (a padded place) gives a row of zeros and takes part in no sum.
  *
- * The reverse adds no floating numbers by atomics, so its results do not change from run to run:
- * the places are sorted by their ids first (a stable radix sort: places of one id stay in order),
- * then chunks of the sorted places are summed in registers, in precision<T>. An id whose places lie
+ * The reverse adds no floating numbers by atomics, so its results do not change from run to run. Up to
+ * DIRECT_MOST places one launch does it all. Beyond, the places are sorted by their ids first (places of
+ * one id stay in order; by counting up to RANK_MOST places, by a stable radix sort beyond), then chunks
+ * of the sorted places are summed in registers, in precision<T>. An id whose places lie
  * within one chunk is written at once; one that crosses chunks leaves a partial row in each, and a
  * last kernel adds those in order. Rows of the table that no id names are cleared (or scaled, by
  * alpha) by workgroups of the same launch as the sums; with alpha = 1 they are not touched. With
@@ -30,6 +31,19 @@ __device__ __forceinline__ unsigned token_key(const void* tokens, bool wide, siz
   return t >= 0 && t < (long long)v ? (unsigned)t : v;
 }
 
+/* Pack p of row `row` of a matrix of `rows` rows of n. The pack that the row's end cuts is read whole too, into
+ * the next row (what is read there is never stored), except where it would pass the matrix's end: a cut pack
+ * read element by element makes its wavefront wait for every row in turn (r16 n = 100, 16000 tokens: the sums
+ * 25 us). */
+template <class T, int W, bool LOOSE, bool NT>
+__device__ __forceinline__ typename vec_of<T, W>::type whole_pack(const RowPacks<T, W, LOOSE>& rp, const T* matrix, size_t row, size_t rows, size_t n, int p) {
+  using VL = typename std::conditional<LOOSE, typename loose_vec_of<T, W>::type, typename vec_of<T, W>::type>::type;
+  const size_t at = row * n + (size_t)(unsigned)p * W;
+  if (LOOSE && at + W > rows * n) return rp.template raw<NT>(matrix + row * n, p);
+  const VL* v = reinterpret_cast<const VL*>(matrix + at);
+  return NT ? __builtin_nontemporal_load(v) : *v;
+}
+
 /* ------------------------------------------------------------------ forward */
 
 /* G lanes hold a strip of G packs of one row, 256 / G rows a workgroup. */
@@ -48,9 +62,9 @@ __global__ __launch_bounds__(256) void embedding_rows(
 #pragma unroll
   for (int i = 0; i < W; ++i) out[i] = (P)0;
   if (k < v) {
-    rp.template load<false>(table + (size_t)k * n, p, out);
+    const typename vec_of<T, W>::type in = whole_pack<T, W, LOOSE, false>(rp, table, k, v, n, p);
 #pragma unroll
-    for (int i = 0; i < W; ++i) out[i] *= scale;
+    for (int i = 0; i < W; ++i) out[i] = (P)in[i] * scale;
   }
   rp.store(y + row * n, p, out);
 }
@@ -317,6 +331,32 @@ __device__ __forceinline__ Run run_around(const unsigned* keys, size_t m, size_t
   return r;
 }
 
+/* Rows [row0, row0 + rows) of the table but those that are named: cleared, or (BLEND) scaled. */
+template <class T, int W, bool BLEND, bool LOOSE>
+__device__ __forceinline__ void clear_unnamed(const RowPacks<T, W, LOOSE>& rp, T* grads, const unsigned* named, size_t row0, unsigned rows, size_t n,
+                                              typename precision<T>::type alpha) {
+  using P = typename precision<T>::type;
+  auto clear = [&](unsigned k, int p) {
+    if (named[k]) return;
+    T* row = grads + (row0 + k) * n;
+    P out[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) out[i] = (P)0;
+    if constexpr (BLEND) {
+      rp.template load<true>(row, p, out);
+#pragma unroll
+      for (int i = 0; i < W; ++i) out[i] *= alpha;
+    }
+    rp.store(row, p, out);
+  };
+  if (rp.npk >= 256) {
+    for (unsigned k = 0; k < rows; ++k)
+      for (int p = threadIdx.x; p < rp.npk; p += 256) clear(k, p);
+  } else { /* several narrow rows at a time */
+    for (unsigned q = threadIdx.x; q < rows * (unsigned)rp.npk; q += 256) clear(q / (unsigned)rp.npk, (int)(q % (unsigned)rp.npk));
+  }
+}
+
 /* Workgroups below sum_blocks: G lanes hold a strip of G packs of the columns and walk one chunk of
  * the sorted places, 256 / G chunks a workgroup. An id of no more places than a chunk belongs to the chunk
  * it begins in, which goes past its end for it; only longer ones are cut where a chunk ends. The others clear (BLEND: scale) the rows of the table
@@ -342,25 +382,7 @@ __global__ __launch_bounds__(256) void embedding_sum(
       named[threadIdx.x] = at < m && keys[at] == key;
     }
     __syncthreads();
-    auto clear = [&](unsigned k, int p) {
-      if (named[k]) return;
-      T* row = grads + (row0 + k) * n;
-      P out[W];
-#pragma unroll
-      for (int i = 0; i < W; ++i) out[i] = (P)0;
-      if constexpr (BLEND) {
-        rp.template load<true>(row, p, out);
-#pragma unroll
-        for (int i = 0; i < W; ++i) out[i] *= alpha;
-      }
-      rp.store(row, p, out);
-    };
-    if (rp.npk >= 256) {
-      for (unsigned k = 0; k < rows; ++k)
-        for (int p = threadIdx.x; p < rp.npk; p += 256) clear(k, p);
-    } else { /* several narrow rows at a time */
-      for (unsigned q = threadIdx.x; q < rows * (unsigned)rp.npk; q += 256) clear(q / (unsigned)rp.npk, (int)(q % (unsigned)rp.npk));
-    }
+    clear_unnamed<T, W, BLEND>(rp, grads, named, row0, rows, n, alpha);
     return;
   }
 
@@ -420,7 +442,7 @@ __global__ __launch_bounds__(256) void embedding_sum(
     for (int u = 0; u < U; ++u) {
       const size_t i = i0 + u < hi ? i0 + u : hi - 1;
       key[u] = keys[i];
-      row[u] = rp.template raw<true>(dy + (size_t)places[i] * n, p);
+      row[u] = whole_pack<T, W, LOOSE, true>(rp, dy, places[i], m, n, p);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -436,6 +458,103 @@ __global__ __launch_bounds__(256) void embedding_sum(
     }
   }
   leave(goes_on);
+}
+
+/* Up to DIRECT_MOST places in one launch and without a workspace: every workgroup has all keys in LDS. A group
+ * of lanes takes a place; where no earlier place has its id, it adds up the rows of that place and of the
+ * later ones, in order, and writes the id's row. The workgroups from `place_blocks` on clear (BLEND: scale)
+ * the rows that no place names. What this saves is two launches, 3.2 us each of the caller's time. */
+constexpr unsigned DIRECT_MOST = 256;
+constexpr int DIRECT_WORDS = DIRECT_MOST / WAVE;
+template <class T, int W, int G, bool BLEND, bool LOOSE>
+__global__ __launch_bounds__(256) void embedding_direct(
+    const void* tokens, unsigned wide, const T* dy, T* grads, typename precision<T>::type scale, typename precision<T>::type alpha, unsigned v, unsigned m,
+    size_t n, unsigned strips, unsigned place_blocks, unsigned fill_rows) {
+  using P = typename precision<T>::type;
+  using V = typename vec_of<T, W>::type;
+  const RowPacks<T, W, LOOSE> rp(n);
+  __shared__ unsigned keys[DIRECT_MOST];
+  const unsigned mine = threadIdx.x < m ? token_key(tokens, wide != 0, threadIdx.x, v) : v;
+
+  if (blockIdx.x >= place_blocks) {
+    __shared__ unsigned named[FILL_MOST];
+    const size_t row0 = (size_t)(blockIdx.x - place_blocks) * fill_rows;
+    const unsigned rows = (unsigned)(v - row0 < fill_rows ? v - row0 : fill_rows);
+    if (threadIdx.x < rows) named[threadIdx.x] = 0;
+    __syncthreads();
+    if (mine >= row0 && mine - row0 < rows) named[mine - row0] = 1; /* v is in no range: row0 + rows <= v */
+    __syncthreads();
+    clear_unnamed<T, W, BLEND>(rp, grads, named, row0, rows, n, alpha);
+    return;
+  }
+  keys[threadIdx.x] = mine;
+  __syncthreads();
+  const int sub = threadIdx.x / G, lane = threadIdx.x % G;
+  const unsigned i = (blockIdx.x / strips) * (256 / G) + sub;
+  const int p = (int)(blockIdx.x % strips) * G + lane;
+  const unsigned key = i < m ? keys[i] : v;
+  /* the places of this group's id, a bit each, by votes of the whole wavefront for each of its groups */
+  unsigned long long places[DIRECT_WORDS];
+#pragma unroll
+  for (int g = 0; g < (G < WAVE ? WAVE / G : 1); ++g) {
+    const unsigned asked = __shfl(key, g * (G < WAVE ? G : 0), WAVE);
+#pragma unroll
+    for (int w = 0; w < DIRECT_WORDS; ++w) {
+      const unsigned long long same = __ballot(keys[w * WAVE + threadIdx.x % WAVE] == asked);
+      if (G >= WAVE || (int)(threadIdx.x % WAVE) / G == g) places[w] = same;
+    }
+  }
+  if (i >= m || p >= rp.npk || key >= v) return;
+  unsigned long long left = 0;
+  bool earlier = false; /* then an earlier place's group adds this one's row */
+#pragma unroll
+  for (int w = 0; w < DIRECT_WORDS; ++w) {
+    const unsigned long long before = i / WAVE > (unsigned)w ? ~0ull : i / WAVE == (unsigned)w ? (1ull << (i % WAVE)) - 1ull : 0ull;
+    earlier = earlier || (places[w] & before) != 0;
+    left |= places[w];
+  }
+  if (earlier) return;
+  P acc[W];
+#pragma unroll
+  for (int e = 0; e < W; ++e) acc[e] = (P)0;
+  constexpr int U = 8;
+  while (left) {
+    unsigned found[U]; /* the next places of the id, the last one again where there are fewer */
+    int count = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      unsigned at = u ? found[u - 1] : 0u;
+#pragma unroll
+      for (int w = DIRECT_WORDS - 1; w >= 0; --w) /* the lowest place that is left */
+        if (places[w]) at = w * WAVE + (unsigned)__builtin_ctzll(places[w]);
+      found[u] = at;
+      count += left ? 1 : 0;
+      left = 0;
+#pragma unroll
+      for (int w = 0; w < DIRECT_WORDS; ++w) {
+        if (at / WAVE == (unsigned)w) places[w] &= ~(1ull << (at % WAVE));
+        left |= places[w];
+      }
+    }
+    V row[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) row[u] = whole_pack<T, W, LOOSE, true>(rp, dy, found[u], m, n, p);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < W; ++e) acc[e] += u < count ? (P)row[u][e] : (P)0;
+  }
+  T* row = grads + (size_t)key * n;
+  P out[W];
+#pragma unroll
+  for (int e = 0; e < W; ++e) out[e] = scale * acc[e];
+  if constexpr (BLEND) {
+    P old[W];
+    rp.template load<true>(row, p, old);
+#pragma unroll
+    for (int e = 0; e < W; ++e) out[e] += alpha * old[e];
+  }
+  rp.store(row, p, out);
 }
 
 /* The ids that cross chunks: the partial rows of each are added up in order, in fp64. Workgroups take (id,
@@ -503,18 +622,14 @@ __global__ __launch_bounds__(256) void embedding_join(
   }
 }
 
-/* alpha * dT without any id */
-template <class T, bool BLEND> __global__ __launch_bounds__(256) void embedding_scale_all(T* grads, typename precision<T>::type alpha, size_t count) {
-  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (i < count) grads[i] = BLEND ? (T)(alpha * (typename precision<T>::type)grads[i]) : (T)0;
-}
-
 /* ------------------------------------------------------------------ host dispatch */
 
-/* The sorted places one chunk holds. */
-inline size_t embedding_chunk(size_t m) {
-  size_t chunk = 8;
-  while (chunk < 32 && m / chunk > 1024) chunk *= 2;
+/* The sorted places one chunk holds: as many as leave the GPU 1024 workgroups, or half of that
+ * for narrow rows, from 4 to 32. */
+inline size_t embedding_chunk(size_t m, size_t row_bytes) {
+  const size_t lanes = (row_bytes + PACK_BYTES - 1) / PACK_BYTES, groups = lanes >= 256 ? 1 : 256 / lanes; /* chunks a workgroup */
+  size_t chunk = 4;
+  while (chunk < 32 && m / chunk > 1024 * (groups < 8 ? groups : 8)) chunk *= 2;
   return chunk;
 }
 
@@ -536,7 +651,7 @@ template <class T> inline EmbeddingScratch embedding_scratch(size_t m, size_t n)
     at += (bytes + 255) / 256 * 256;
     return here;
   };
-  const size_t chunk = embedding_chunk(m), chunks = (m + chunk - 1) / chunk, pairs = m > RANK_MOST ? 2 : 1;
+  const size_t chunk = embedding_chunk(m, n * sizeof(T)), chunks = (m + chunk - 1) / chunk, pairs = m > RANK_MOST ? 2 : 1;
   for (size_t k = 0; k < pairs; ++k) {
     s.keys[k] = take(m * sizeof(unsigned));
     s.places[k] = take(m * sizeof(unsigned));
@@ -594,17 +709,28 @@ inline void embedding_reverse(const void* tokens, const T* dy, T* grads, void* s
   constexpr int W = PACK_BYTES / (int)sizeof(T);
   embedding_check(tokens, id_bytes, v, m, n);
   if (v == 0 || n == 0) return;
-  if (m == 0) {
-    if (alpha == 1.0) return;
-    const size_t count = v * n, blocks = (count + 255) / 256;
-    require(blocks < 0x7fffffffull, "embedding reverse: table too large for one grid");
-    if (alpha == 0.0) embedding_scale_all<T, false><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(grads, (P)alpha, count);
-    else embedding_scale_all<T, true><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(grads, (P)alpha, count);
+  require(m == 0 || scratch != nullptr, "embedding reverse: scratch must hold mpEmbeddingReverseScratchBytes bytes");
+  require(reinterpret_cast<uintptr_t>(scratch) % 16 == 0, "embedding reverse: scratch must be 16-byte aligned");
+  const bool loose = !(aligned16(dy) && aligned16(grads) && n % W == 0);
+  const size_t packs = (n + W - 1) / W;
+  const unsigned wide = id_bytes == 8, fill_rows = embedding_fill_rows(n * sizeof(T));
+  if (m <= DIRECT_MOST) {
+    const size_t fill = alpha == 1.0 ? 0 : (v + fill_rows - 1) / fill_rows;
+    for_strip(packs, [&]<int G>() {
+      const size_t strips = (packs + G - 1) / G, places = (m + 256 / G - 1) / (256 / G) * strips;
+      require(places + fill < 0x7fffffffull, "embedding reverse: too many rows for one grid");
+      if (places + fill == 0) return; /* no token, and nothing to clear or to scale */
+      const dim3 grid((unsigned)(places + fill)), block(256);
+      auto go = [&]<bool BLEND, bool LOOSE>() {
+        embedding_direct<T, W, G, BLEND, LOOSE><<<grid, block, 0, stream>>>(tokens, wide, dy, grads, (P)scale, (P)alpha, (unsigned)v, (unsigned)m, n,
+                                                                            (unsigned)strips, (unsigned)places, fill_rows);
+      };
+      if (alpha != 0.0) { if (loose) go.template operator()<true, true>(); else go.template operator()<true, false>(); }
+      else { if (loose) go.template operator()<false, true>(); else go.template operator()<false, false>(); }
+    });
     MP_CHECK_LAUNCH();
     return;
   }
-  require(scratch != nullptr, "embedding reverse: scratch must hold mpEmbeddingReverseScratchBytes bytes");
-  require(reinterpret_cast<uintptr_t>(scratch) % 16 == 0, "embedding reverse: scratch must be 16-byte aligned");
   const EmbeddingScratch at = embedding_scratch<T>(m, n);
   char* base = static_cast<char*>(scratch);
   auto words = [&](size_t offset) { return reinterpret_cast<unsigned*>(base + offset); };
@@ -613,7 +739,6 @@ inline void embedding_reverse(const void* tokens, const T* dy, T* grads, void* s
   P* partials = reinterpret_cast<P*>(base + at.partials);
 
   /* the sort, with a part of the clearing in each of its launches */
-  const unsigned wide = id_bytes == 8;
   const int passes = sort_passes(v);
   const size_t unit = (size_t)SORT_THREADS * FILL_PACKS * W; /* elements a clearing workgroup of a sort's launch takes */
   const size_t elements = alpha == 0.0 ? v * n : 0;
@@ -654,10 +779,8 @@ inline void embedding_reverse(const void* tokens, const T* dy, T* grads, void* s
     sorted_places = places[(passes - 1) & 1];
   }
 
-  const bool loose = !(aligned16(dy) && aligned16(grads) && n % W == 0);
-  const size_t packs = (n + W - 1) / W, chunk = embedding_chunk(m), chunks = (m + chunk - 1) / chunk;
+  const size_t chunk = embedding_chunk(m, n * sizeof(T)), chunks = (m + chunk - 1) / chunk;
   const size_t row_begin = cleared / n; /* rows from here on are still to be looked at, the first of them perhaps half cleared */
-  const unsigned fill_rows = embedding_fill_rows(n * sizeof(T));
   const size_t fill = alpha == 1.0 ? 0 : (v - row_begin + fill_rows - 1) / fill_rows;
   for_strip(packs, [&]<int G>() {
     const size_t strips = (packs + G - 1) / G, sums = (chunks + 256 / G - 1) / (256 / G) * strips;

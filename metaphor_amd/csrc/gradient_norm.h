@@ -24,6 +24,9 @@
 
 #include "row_dispatch.h"
 
+#include <stdlib.h>
+#include <algorithm>
+
 #if defined(__cplusplus) && defined(__HIPCC__)
 
 namespace mp {
@@ -32,7 +35,7 @@ constexpr int NORM_RUNS = 120, NORM_THREADS = 256, NORM_PACKS = 4;
 constexpr size_t NORM_PIECE = (size_t)NORM_THREADS * NORM_PACKS * PACK_BYTES, NORM_PARTIALS = 1024; /* a table */
 /* up to so many pieces the scaling adds up the partial sums itself, in every workgroup, and one launch is
  * saved; beyond, a workgroup would spend as long on that as on its piece */
-constexpr size_t NORM_FUSED_PIECES = 1024;
+constexpr size_t NORM_FUSED_PIECES = 2048;
 
 constexpr size_t NORM_KEPT_BYTES = (size_t)224 << 20, NORM_KEPT_PIECES = NORM_KEPT_BYTES / NORM_PIECE;
 
@@ -70,6 +73,15 @@ template <class T> struct NormPiece {
   }
   __device__ __forceinline__ size_t at(int u) const { return ((size_t)u * NORM_THREADS + threadIdx.x) * W; }
   __device__ __forceinline__ bool whole() const { return left >= LEN; }
+  /* pack u where the run ends in this piece: zeros past its end */
+  template <int WIDTH> __device__ __forceinline__ typename vec_of<T, WIDTH>::type cut(const T* src, int u) const {
+    typename vec_of<T, WIDTH>::type v;
+    const size_t i = at(u);
+    if (i + WIDTH <= left) return *reinterpret_cast<const typename loose_vec_of<T, WIDTH>::type*>(src + i);
+#pragma unroll
+    for (int j = 0; j < WIDTH; ++j) v[j] = i + j < left ? src[i + j] : (T)0;
+    return v;
+  }
 };
 
 /* Sum over the workgroup's threads; every thread gets it. */
@@ -100,8 +112,14 @@ template <bool KEEP, class T> __device__ __forceinline__ double piece_squares(co
     for (int u = 0; u < NORM_PACKS; ++u)
 #pragma unroll
       for (int j = 0; j < W; ++j) s += (double)v[u][j] * (double)v[u][j];
-  } else {
-    for (size_t i = threadIdx.x; i < piece.left; i += NORM_THREADS) s += (double)src[i] * (double)src[i];
+  } else { /* the run's last piece: the packs that exist, and the elements behind the last one */
+    typename vec_of<T, W>::type v[NORM_PACKS];
+#pragma unroll
+    for (int u = 0; u < NORM_PACKS; ++u) v[u] = piece.template cut<W>(src, u);
+#pragma unroll
+    for (int u = 0; u < NORM_PACKS; ++u)
+#pragma unroll
+      for (int j = 0; j < W; ++j) s += (double)v[u][j] * (double)v[u][j];
   }
   return s;
 }
@@ -145,9 +163,13 @@ __global__ __launch_bounds__(NORM_THREADS) void gradient_scaled(NormTable<T> t, 
   T* dst = t.dst[piece.run] + piece.lo;
   typename vec_of<T, W>::type v[NORM_PACKS];
   const bool whole = piece.whole();
-  if (whole)
+  if (whole) {
 #pragma unroll
     for (int u = 0; u < NORM_PACKS; ++u) v[u] = __builtin_nontemporal_load(reinterpret_cast<const VL*>(src + piece.at(u)));
+  } else {
+#pragma unroll
+    for (int u = 0; u < NORM_PACKS; ++u) v[u] = piece.template cut<W>(src, u);
+  }
   double total;
   if constexpr (FUSED) {
     __shared__ double slots[NORM_THREADS / WAVE];
@@ -159,16 +181,19 @@ __global__ __launch_bounds__(NORM_THREADS) void gradient_scaled(NormTable<T> t, 
   const bool within = total <= max_norm;
   if (src == dst && within) return; /* nothing to do in place */
   const P factor = within ? (P)1 : (P)(max_norm / total);
-  if (whole) {
 #pragma unroll
-    for (int u = 0; u < NORM_PACKS; ++u) {
-      P out[W];
+  for (int u = 0; u < NORM_PACKS; ++u) {
+    const size_t i = piece.at(u);
+    P out[W];
 #pragma unroll
-      for (int j = 0; j < W; ++j) out[j] = (P)v[u][j] * factor;
-      store_pack_nt_loose<T, W>(dst + piece.at(u), out);
+    for (int j = 0; j < W; ++j) out[j] = (P)v[u][j] * factor;
+    if (whole || i + W <= piece.left) {
+      store_pack_nt_loose<T, W>(dst + i, out);
+    } else {
+#pragma unroll
+      for (int j = 0; j < W; ++j)
+        if (i + j < piece.left) dst[i + j] = (T)out[j];
     }
-  } else {
-    for (size_t i = threadIdx.x; i < piece.left; i += NORM_THREADS) dst[i] = (T)((P)src[i] * factor);
   }
 }
 
@@ -255,6 +280,40 @@ inline void gradient_check_limit(const void* outs, double max_norm, size_t count
   require(max_norm >= 0.0, "gradient clip: the largest norm must not be negative or NaN");
 }
 
+/* A tensor listed twice, or a result that reaches into another tensor, would be scaled once or twice as the
+ * workgroups happen to run: refused. A result is its own gradient or clear of all of them. Results in rising
+ * order (a bucket's) are checked in one walk, others are ordered first. */
+template <class T> inline void gradient_check_apart(const void* const* grads, const void* const* outs, const len_t* sizes, size_t count) {
+  struct Span { uintptr_t begin, end; };
+  auto span = [&](const void* const* a, size_t k) { const uintptr_t at = reinterpret_cast<uintptr_t>(a[k]); return Span{at, at + sizes[k] * sizeof(T)}; };
+  const char* twice = "gradient clip: a result overlaps another result or another gradient";
+  bool rising = true, in_place = true;
+  uintptr_t end = 0;
+  for (size_t k = 0; k < count; ++k) {
+    if (sizes[k] == 0) continue;
+    const Span s = span(outs, k);
+    rising = rising && s.begin >= end;
+    in_place = in_place && grads[k] == outs[k];
+    end = s.end;
+  }
+  if (rising && in_place) return;
+  Span* spans = static_cast<Span*>(::malloc(count * sizeof(Span)));
+  require(spans != nullptr, "gradient clip: out of host memory");
+  size_t used = 0;
+  for (size_t k = 0; k < count; ++k)
+    if (sizes[k]) spans[used++] = span(outs, k);
+  const auto before = [](const Span& a, const Span& b) { return a.begin < b.begin; };
+  if (!rising) std::sort(spans, spans + used, before);
+  for (size_t k = 1; k < used; ++k) require(spans[k - 1].end <= spans[k].begin, twice);
+  for (size_t k = 0; k < count && !in_place; ++k) {
+    if (sizes[k] == 0 || grads[k] == outs[k]) continue;
+    const Span s = span(grads, k);
+    const Span* behind = std::lower_bound(spans, spans + used, Span{s.end, 0}, before); /* the first that begins at its end or later */
+    require(behind == spans || behind[-1].end <= s.begin, twice);
+  }
+  ::free(spans);
+}
+
 /* returns how many partial sums there are */
 template <class T>
 inline unsigned gradient_squares_all(const void* const* grads, const len_t* sizes, double* partials, size_t count, hipStream_t stream) {
@@ -294,6 +353,7 @@ template <class T>
 inline void gradient_scale(const void* grads, const void* outs, const void* sizes, const void* norm, double max_norm, size_t count, hipStream_t stream) {
   gradient_check_limit(outs, max_norm, count);
   gradient_check<T>(grads, outs, sizes, norm, count);
+  gradient_check_apart<T>(static_cast<const void* const*>(grads), static_cast<const void* const*>(outs), static_cast<const len_t*>(sizes), count);
   gradient_scale_all<T>(static_cast<const void* const*>(grads), static_cast<const void* const*>(outs), static_cast<const len_t*>(sizes),
                         static_cast<const double*>(norm), 0, nullptr, max_norm, count, stream);
 }
@@ -306,6 +366,7 @@ inline void gradient_clip(const void* grads, const void* outs, const void* sizes
   gradient_check_scratch(scratch, count);
   const void* const* src = static_cast<const void* const*>(grads);
   const void* const* dst = static_cast<const void* const*>(outs);
+  gradient_check_apart<T>(src, dst, static_cast<const len_t*>(sizes), count);
   const len_t* lengths = static_cast<const len_t*>(sizes);
   double *partials = static_cast<double*>(scratch), *out = static_cast<double*>(norm);
   const unsigned used = gradient_squares_all<T>(src, lengths, partials, count, stream);

@@ -7,7 +7,7 @@
 //   bias_grads[j]  = sum_i dst_grads[i,j]                                       + alpha*bias_grads[j]
 // gain_grads or bias_grads that is NULL is not computed; src_grads may be dst_grads or src. alpha = 0
 // never reads the three results. scratch is caller-owned workspace of
-// mpLayernormReverseScratchBytes(dtype, m, n) bytes (the reference hands kernels their workspace from
+// mpLayernormReverseScratchBytes(dtype, m, n) bytes, 16-byte aligned (the reference hands kernels their workspace from
 // the per-stream scratch, src/core/utils.zig:20-36). Results do not change from run to run.
 extern "C" void launch_layernorm_ij_j_reverse_Scalar(
   const void* src,

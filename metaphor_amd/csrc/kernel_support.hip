@@ -65,8 +65,8 @@ extern "C" len_t mpReduceScratchBytes(len_t dtype, len_t m, len_t n) {
 }
 
 // Bytes of caller-owned scratch that launch_layernorm_ij_j_reverse_<dtype> needs for an [m, n] problem:
-// two rows of n accumulators (for the gain and the bias) per workgroup, at most two workgroups per
-// compute unit.
+// two rows of accumulators (for the gain and the bias, n of them rounded up to whole 16-byte packs of the
+// dtype) per workgroup, at most two workgroups per compute unit.
 extern "C" len_t mpLayernormReverseScratchBytes(len_t dtype, len_t m, len_t n) {
   switch (dtype) {
     case MP_R16: return mp::layernorm_reverse_scratch_bytes<r16>(m, n);

@@ -21,6 +21,13 @@
 
 namespace mp {
 
+/* A partial row holds dg's sums from its start and db's from partial_apart on: n rounded up to whole packs of
+ * T, so that packs of sums are stored and added whole and aligned. */
+template <class T> __host__ __device__ inline size_t partial_apart(size_t n) {
+  constexpr size_t W = PACK_BYTES / sizeof(T);
+  return (n + W - 1) / W * W;
+}
+
 /* The variance from mean((x - c)^2) and mean(x - c): never below zero by rounding, NaN kept. */
 template <class P> __device__ __forceinline__ P variance_of(P square, P off) {
   const P v = square - off * off;
@@ -81,8 +88,8 @@ __global__ __launch_bounds__(STREAM_THREADS) void layernorm_fwd_stream(
 }
 
 /* The reverse of the same: the mean, then the variance with both of the gradient's row sums, then the
- * write. A workgroup walks rows and keeps its sums for dg and db in a partial row of 2n values of
- * its own, where a column always belongs to the same thread. */
+ * write. A workgroup walks rows and keeps its sums for dg and db in a partial row of its own, where a
+ * column always belongs to the same thread. */
 template <class T, int W, bool BLEND, bool LOOSE>
 __global__ __launch_bounds__(STREAM_THREADS) void layernorm_rev_stream(
     const T* x, const T* gain, const T* dy, T* dx, typename precision<T>::type* partials,
@@ -93,7 +100,8 @@ __global__ __launch_bounds__(STREAM_THREADS) void layernorm_rev_stream(
   const P inv_n = (P)1 / (P)n;
   const int lane = threadIdx.x;
   const RowPacks<T, W, LOOSE> rp(n);
-  P* mine = partials + (size_t)blockIdx.x * 2 * n;
+  const size_t apart = partial_apart<T>(n);
+  P* mine = partials + (size_t)blockIdx.x * 2 * apart;
   bool first = true;
   for (size_t row = blockIdx.x; row < m; row += gridDim.x, first = false) {
     const T* xr = x + row * n;
@@ -149,7 +157,7 @@ __global__ __launch_bounds__(STREAM_THREADS) void layernorm_rev_stream(
         if (i < rp.valid(p)) {
           P* at = mine + (size_t)p * W + i;
           at[0] = (first ? (P)0 : at[0]) + d[i] * h;
-          at[n] = (first ? (P)0 : at[n]) + d[i];
+          at[apart] = (first ? (P)0 : at[apart]) + d[i];
         }
       }
       rp.store(out_row, p, out);
@@ -507,10 +515,11 @@ __global__ __launch_bounds__(NORM_BLOCK) void layernorm_fwd_rows(
 /* Persistent workgroups walk the rows; with PAIR the next rows' x and dy are on their way (into a second
  * set of registers) while these are reduced, behind a barrier that orders LDS traffic only, and written.
  * The columns' sums for dg and db stay in registers; at the end the rows of a workgroup are folded in
- * order and it leaves ONE partial row of 2n sums. BLOCK 512 leaves a lane 256 registers. */
+ * order and it leaves ONE partial row, or, where it is the only workgroup, dg and db themselves. BLOCK 512
+ * leaves a lane 256 registers. */
 template <class T, int W, int SUB, int NV, bool BLEND, bool LOOSE, bool PAIR, int BLOCK>
 __global__ __launch_bounds__(BLOCK) void layernorm_rev_rows(
-    const T* x, const T* gain, const T* dy, T* dx, typename precision<T>::type* partials,
+    const T* x, const T* gain, const T* dy, T* dx, T* dg, T* db, typename precision<T>::type* partials,
     typename precision<T>::type eps, typename precision<T>::type alpha, size_t m, size_t n, int gw) {
   using P = typename precision<T>::type;
   using Row = NormRow<T, W, SUB, NV, LOOSE>;
@@ -618,6 +627,7 @@ __global__ __launch_bounds__(BLOCK) void layernorm_rev_rows(
       fetch(bx, bd, base + stride);
       __builtin_amdgcn_sched_barrier(0);
       finish(ax, ad, base, parts[0]);
+      if (base + stride >= m) break;
       fetch(ax, ad, base + 2 * stride);
       __builtin_amdgcn_sched_barrier(0);
       finish(bx, bd, base + stride, parts[1]);
@@ -633,7 +643,32 @@ __global__ __launch_bounds__(BLOCK) void layernorm_rev_rows(
   /* the rows of a wavefront, then the row groups of the workgroup, a pack of every lane at a time */
   const int groups = SUB < WAVE ? (int)blockDim.x / WAVE : at.rows_here;
   const int width = at.G; /* lanes a group */
-  P* out = partials + (size_t)blockIdx.x * 2 * n;
+  const size_t apart = partial_apart<T>(n);
+  P* out = partials + (size_t)blockIdx.x * 2 * apart;
+  /* a pack of sums of column p * W on; `alone`: in the results' type, added to what they hold */
+  const bool alone = gridDim.x == 1;
+  auto leave = [&](int which, int p, const P (&a)[W]) {
+    if (!alone) {
+#pragma unroll
+      for (int i = 0; i < W; i += PACK_BYTES / (int)sizeof(P)) {
+        P some[PACK_BYTES / sizeof(P)];
+#pragma unroll
+        for (int j = 0; j < PACK_BYTES / (int)sizeof(P); ++j) some[j] = a[i + j];
+        store_pack<P, PACK_BYTES / (int)sizeof(P)>(out + which * apart + (size_t)p * W + i, some);
+      }
+      return;
+    }
+    T* to = which ? db : dg;
+    if (!to) return;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      if (i >= rw.rp.valid(p)) break;
+      T* cell = to + (size_t)p * W + i;
+      double t = (double)a[i];
+      if constexpr (BLEND) t += (double)alpha * (double)*cell;
+      *cell = (T)t;
+    }
+  };
 #pragma unroll
   for (int k = 0; k < NV; ++k)
 #pragma unroll
@@ -646,12 +681,7 @@ __global__ __launch_bounds__(BLOCK) void layernorm_rev_rows(
           for (int step = SUB; step < WAVE; step <<= 1) a[i] += __shfl_xor(a[i], step, WAVE);
       }
       if (groups == 1) {
-        if (rw.inside(k)) {
-          const int p = rw.pack(k);
-#pragma unroll
-          for (int i = 0; i < W; ++i)
-            if (i < rw.rp.valid(p)) out[which * n + (size_t)p * W + i] = a[i];
-        }
+        if (rw.inside(k)) leave(which, rw.pack(k), a);
         continue;
       }
       const int group = SUB < WAVE ? (int)threadIdx.x / WAVE : at.sub, l = threadIdx.x % width;
@@ -660,41 +690,43 @@ __global__ __launch_bounds__(BLOCK) void layernorm_rev_rows(
 #pragma unroll
         for (int i = 0; i < W; ++i) comb[(group * width + l) * W + i] = a[i];
       __syncthreads();
-      for (int c = threadIdx.x; c < width * W; c += blockDim.x) {
-        const size_t col = (size_t)k * width * W + c;
-        if (col < n) {
-          P t = (P)0;
-          for (int g = 0; g < groups; ++g) t += comb[g * width * W + c];
-          out[which * n + col] = t;
-        }
+      const int p = k * width + (int)threadIdx.x;
+      if ((int)threadIdx.x < width && p < rw.rp.npk) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) a[i] = (P)0;
+        for (int g = 0; g < groups; ++g)
+#pragma unroll
+          for (int i = 0; i < W; ++i) a[i] += comb[(g * width + threadIdx.x) * W + i];
+        leave(which, p, a);
       }
     }
 }
 
 /* ------------------------------------------------------------------ dg and db from the partial rows */
 
-/* The partial rows (2n columns: dg's, then db's) added in a fixed order in fp64. A workgroup owns
- * FINISH_COLS columns, FINISH_SLICES slices of it take the rows in turn with eight loads on their way. */
+/* The partial rows added in a fixed order in fp64. A workgroup owns a 128-byte line of columns; its 64 slices
+ * take the rows in turn, a 16-byte load of eight rows on its way at once. */
 constexpr int NORM_FINISH_LANES = 8, NORM_FINISH_SLICES = 64;
-template <class T, int CW>
+template <class T>
 __global__ __launch_bounds__(NORM_FINISH_LANES * NORM_FINISH_SLICES) void layernorm_grads_finish(
     const typename precision<T>::type* partials, T* dg, T* db, double alpha, int rows, size_t n) {
   using P = typename precision<T>::type;
-  constexpr int COLS = NORM_FINISH_LANES * CW;
+  constexpr int CW = PACK_BYTES / (int)sizeof(P), COLS = NORM_FINISH_LANES * CW;
   __shared__ double part[NORM_FINISH_SLICES][COLS + 1];
   const int c = threadIdx.x % NORM_FINISH_LANES, slice = threadIdx.x / NORM_FINISH_LANES;
-  const size_t col = ((size_t)blockIdx.x * NORM_FINISH_LANES + c) * CW, width = 2 * n;
+  const size_t apart = partial_apart<T>(n), width = 2 * apart;
+  const size_t col = ((size_t)blockIdx.x * NORM_FINISH_LANES + c) * CW;
   double s[CW];
 #pragma unroll
   for (int i = 0; i < CW; ++i) s[i] = 0.0;
-  if (col < width) { /* 2n is a multiple of CW */
+  if (col < width) { /* a whole number of packs */
     constexpr int U = 8;
     for (int p = slice; p < rows; p += U * NORM_FINISH_SLICES) {
       P v[U][CW];
 #pragma unroll
-      for (int u = 0; u < U; ++u) { /* beyond the last row: the last, left out */
+      for (int u = 0; u < U; ++u) { /* beyond the last row: this slice's first, left out */
         const int q = p + u * NORM_FINISH_SLICES;
-        load_pack<P, CW>(partials + (size_t)(q < rows ? q : rows - 1) * width + col, v[u]);
+        load_pack<P, CW>(partials + (size_t)(q < rows ? q : p) * width + col, v[u]);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -705,11 +737,11 @@ __global__ __launch_bounds__(NORM_FINISH_LANES * NORM_FINISH_SLICES) void layern
 #pragma unroll
   for (int i = 0; i < CW; ++i) part[slice][c * CW + i] = s[i];
   __syncthreads();
-  const size_t at = (size_t)blockIdx.x * COLS + threadIdx.x;
-  if (threadIdx.x < COLS && at < width) {
-    T* out = at < n ? dg : db;
+  const size_t at = (size_t)blockIdx.x * COLS + threadIdx.x, j = at < apart ? at : at - apart;
+  if (threadIdx.x < COLS && at < width && j < n) {
+    T* out = at < apart ? dg : db;
     if (!out) return;
-    out += at < n ? at : at - n;
+    out += j;
     double t = 0.0;
 #pragma unroll 8
     for (int i = 0; i < NORM_FINISH_SLICES; ++i) t += part[i][threadIdx.x];
@@ -727,7 +759,7 @@ inline size_t layernorm_partial_rows(size_t m) {
 }
 
 template <class T> inline size_t layernorm_reverse_scratch_bytes(size_t m, size_t n) {
-  return layernorm_partial_rows(m) * 2 * n * sizeof(typename precision<T>::type);
+  return layernorm_partial_rows(m) * 2 * partial_apart<T>(n) * sizeof(typename precision<T>::type);
 }
 
 /* How a launch holds its rows: `sub` lanes a row below 64, else `gw` wavefronts, `nv` packs a lane, `rows`
@@ -833,11 +865,13 @@ inline void layernorm_reverse_as(const NormPlan& plan, const T* x, const T* gain
       else { if (loose) go.template operator()<false, true>(); else go.template operator()<false, false>(); }
     } else {
       rows = norm_grid(plan, m);
+      /* a few rows: one workgroup takes them all, and one launch is saved */
+      if (rows <= 2) rows = 1;
       require(rows <= layernorm_partial_rows(m), "layernorm reverse: more partial rows than the workspace holds");
       const dim3 grid((unsigned)rows), block(norm_block(plan));
       auto go = [&]<int SUB, int NV, bool PAIR, int BLOCK>() {
         auto as = [&]<bool BLEND, bool LOOSE>() {
-          layernorm_rev_rows<T, W, SUB, NV, BLEND, LOOSE, PAIR, BLOCK><<<grid, block, 0, stream>>>(x, gain, dy, dx, partials, (P)eps, (P)alpha, m, n, plan.gw);
+          layernorm_rev_rows<T, W, SUB, NV, BLEND, LOOSE, PAIR, BLOCK><<<grid, block, 0, stream>>>(x, gain, dy, dx, dg, db, partials, (P)eps, (P)alpha, m, n, plan.gw);
         };
         if (alpha != 0.0) { if (loose) as.template operator()<true, true>(); else as.template operator()<true, false>(); }
         else { if (loose) as.template operator()<false, true>(); else as.template operator()<false, false>(); }
@@ -859,13 +893,10 @@ inline void layernorm_reverse_as(const NormPlan& plan, const T* x, const T* gain
     }
     MP_CHECK_LAUNCH();
   }
-  if (!dg && !db) return;
-  /* wide loads need 16-byte aligned partial rows: fp32 sums, 2n % 4 == 0, an aligned workspace */
-  const bool wide = sizeof(P) == 4 && n % 2 == 0 && aligned16(partials);
-  const size_t cols = wide ? NORM_FINISH_LANES * 4 : NORM_FINISH_LANES;
-  const dim3 grid((unsigned)((2 * n + cols - 1) / cols)), block(NORM_FINISH_LANES * NORM_FINISH_SLICES);
-  if (wide) { if constexpr (sizeof(P) == 4) layernorm_grads_finish<T, 4><<<grid, block, 0, stream>>>(partials, dg, db, alpha, (int)rows, n); }
-  else layernorm_grads_finish<T, 1><<<grid, block, 0, stream>>>(partials, dg, db, alpha, (int)rows, n);
+  if ((!dg && !db) || (m > 0 && plan.nv != 0 && rows == 1)) return;
+  constexpr size_t cols = NORM_FINISH_LANES * PACK_BYTES / sizeof(P);
+  const dim3 grid((unsigned)((2 * partial_apart<T>(n) + cols - 1) / cols)), block(NORM_FINISH_LANES * NORM_FINISH_SLICES);
+  layernorm_grads_finish<T><<<grid, block, 0, stream>>>(partials, dg, db, alpha, (int)rows, n);
   MP_CHECK_LAUNCH();
 }
 
@@ -877,7 +908,7 @@ inline void layernorm_reverse(const T* x, const T* gain, const T* dy, T* dx, T* 
   require(n <= 0x40000000ull, "layernorm reverse: row length must not exceed 2^30");
   require(dg != db || dg == nullptr, "layernorm reverse: gain_grads and bias_grads must be different vectors");
   require(m == 0 || scratch != nullptr, "layernorm reverse: scratch must hold mpLayernormReverseScratchBytes bytes");
-  require(reinterpret_cast<uintptr_t>(scratch) % sizeof(typename precision<T>::type) == 0, "layernorm reverse: scratch must be aligned to its sums");
+  require(reinterpret_cast<uintptr_t>(scratch) % 16 == 0, "layernorm reverse: scratch must be aligned to its sums in packs (16-byte aligned)");
   layernorm_reverse_as<T>(layernorm_reverse_plan<T>((n + W - 1) / W), x, gain, dy, dx, dg, db, scratch, eps, alpha, m, n, stream);
 }
 

@@ -217,3 +217,24 @@ def test_the_gradient_agrees_with_differences():
     lookup(table + way, tokens, up, 3.0)
     lookup(table - way, tokens, down, 3.0)
     assert abs(float(((up - down) * dy).sum()) / 2 - float((dt * way).sum())) < 1e-9
+
+
+@pytest.mark.parametrize("m", [1, 2, 31, 33, 64, 127, 128, 129, 200, 255, 256, 257])
+@pytest.mark.parametrize("kind", KINDS)
+def test_few_tokens(m, kind):
+    """Around a wavefront's votes and what one launch without a workspace takes; rows of one pack to several strips."""
+    for dtype, n in ((F16, 5), (F32, 36), (F64, 130), (F16, 1000), (F32, 1500)):
+        for v, alpha in ((1, 0.0), (90, 0.5), (700, 0.0)):
+            check(dtype, kind, v, m, n, scale=0.5, alpha=alpha, wide=m % 2 == 0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [1, 24, 77, 2048])
+def test_no_token_scales_the_gradient(dtype, n):
+    v, old = 37, normal((37, n), dtype, 5)
+    none = torch.empty(0, dtype=torch.int64, device="cuda")
+    for alpha in (0.0, 1.0, -0.25):
+        dt = guarded(old if alpha else torch.full_like(old, float("nan")))
+        G._call("embedding_i_ij_reverse", dtype, none.data_ptr(), None, dt.t.data_ptr(), None, 2.0, alpha, 8, v, 0, n)
+        assert torch.equal(dt.t.cpu(), (old.double() * alpha).to(dtype)), f"{dtype} n={n} alpha={alpha}"
+        dt.check(f"no token {dtype} n={n} alpha={alpha}")

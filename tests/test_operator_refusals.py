@@ -16,6 +16,7 @@ CASES = [
     ("layernorm_ij_j_reverse", f"{FAKE}, {FAKE}, {FAKE}, {FAKE}, {FAKE}, {FAKE}, {FAKE}, 1e-5, 0.0, 4, (1 << 30) + 1", "row length must not exceed"),
     ("layernorm_ij_j_reverse", f"{FAKE}, {FAKE}, {FAKE}, {FAKE}, {FAKE}, {FAKE}, {FAKE + 64}, 1e-5, 0.0, 4, 64", "must be different vectors"),
     ("layernorm_ij_j_reverse", f"{FAKE}, {FAKE}, {FAKE}, {FAKE}, {FAKE}, {FAKE + 512}, {FAKE + 2}, 1e-5, 0.0, 4, 64", "aligned to its sums"),
+    ("layernorm_ij_j_reverse", f"{FAKE}, {FAKE}, {FAKE}, {FAKE}, {FAKE}, {FAKE + 512}, {FAKE + 8}, 1e-5, 0.0, 4, 64", "16-byte aligned"),
     ("embedding_i_ij", f"{FAKE}, {FAKE}, {FAKE}, 1.0, 2, 10, 4, 64", "4 or 8 bytes wide"),
     ("embedding_i_ij", f"{FAKE}, {FAKE + 4}, {FAKE}, 1.0, 8, 10, 4, 64", "aligned to their width"),
     ("embedding_i_ij", f"{FAKE}, {FAKE}, {FAKE}, 1.0, 8, (1 << 32) - 1, 4, 64", "fewer than 2^32 - 1 rows"),
@@ -34,6 +35,11 @@ CASES = [
     ("gradient_scale", f"A({FAKE}), A(None), L(5), {FAKE}, 1.0, 1", "address is NULL"),
     ("gradient_scale", f"A({FAKE}), A({FAKE}), L(5), {FAKE}, -1.0, 1", "must not be negative"),
     ("gradient_clip", f"A({FAKE}), A({FAKE}), L(5), {FAKE}, {FAKE}, float('nan'), 1", "must not be negative"),
+    ("gradient_clip", f"A({FAKE}, {FAKE}), A({FAKE}, {FAKE}), L(5, 5), {FAKE}, {FAKE}, 1.0, 2", "overlaps another"),
+    ("gradient_clip", f"A({FAKE}, {FAKE + 64}), A({FAKE + 128}, {FAKE + 144}), L(5, 5), {FAKE}, {FAKE}, 1.0, 2", "overlaps another"),
+    ("gradient_clip", f"A({FAKE}, {FAKE + 64}), A({FAKE + 256}, {FAKE + 4}), L(5, 5), {FAKE}, {FAKE}, 1.0, 2", "overlaps another"),
+    ("gradient_scale", f"A({FAKE}), A({FAKE + 16}), L(5), {FAKE}, 1.0, 1", "overlaps another"),
+    ("gradient_scale", f"A({FAKE + 512}, {FAKE}, {FAKE + 100}), A({FAKE + 512}, {FAKE}, {FAKE + 100}), L(5, 26, 5), {FAKE}, 1.0, 3", "overlaps another"),
 ]
 
 
