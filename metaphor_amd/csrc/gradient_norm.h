@@ -11,11 +11,12 @@
  * and sizes travel as kernel arguments, NORM_RUNS of them a launch: nothing is copied to the device and a
  * captured launch keeps its own table. A table's work is cut into pieces of NORM_PIECE bytes, four 16-byte
  * packs a thread; workgroups take them in turn for the squares, each leaving one partial sum in the
- * workspace, and one each for the scaling.
+ * workspace, and one each for the scaling (1024 workgroups for the squares: 203 M elements in 400 tensors 419 us
+ * to clip, 2048 425, 100 tensors of 1000 elements the norm 6.4 and 7.0).
  *
  * The squares are bound by reading the tensors once, the scaling by reading and writing them once. r32,
- * 203 M elements: squares 124 us (6.6 TB/s), both together 365 us, of which the scaling on its own would
- * take 259: the squares read the last NORM_KEPT_BYTES through loads that leave them in the 256 MiB
+ * 203 M elements: squares 124 us (6.6 TB/s), both together 367 us, of which the scaling on its own would
+ * take 262: the squares read the last NORM_KEPT_BYTES through loads that leave them in the 256 MiB
  * memory-side cache, where the scaling finds them (all of it through such loads: squares 136 us,
  * together 375; none: 122 and 387; the scaling from the end backwards: 375).
  */
@@ -161,33 +162,47 @@ __global__ __launch_bounds__(NORM_THREADS) void gradient_scaled(NormTable<T> t, 
   const NormPiece<T> piece(t, blockIdx.x);
   const T* src = t.src[piece.run] + piece.lo;
   T* dst = t.dst[piece.run] + piece.lo;
+  /* what to scale by; false: nothing to do in place */
+  auto factor_of = [&](P& factor) {
+    double total;
+    if constexpr (FUSED) {
+      __shared__ double slots[NORM_THREADS / WAVE];
+      total = ::sqrt(norm_of(norm_in, partials, slots));
+      if (blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = total;
+    } else {
+      total = norm_in[0];
+    }
+    const bool within = total <= max_norm;
+    factor = within ? (P)1 : (P)(max_norm / total);
+    return !(within && src == dst);
+  };
   typename vec_of<T, W>::type v[NORM_PACKS];
-  const bool whole = piece.whole();
-  if (whole) {
+  P factor;
+  auto scaled = [&](int u, P (&out)[W]) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) out[j] = (P)v[u][j] * factor;
+  };
+  if (piece.whole()) { /* on its own from load to store: 203 M elements 262 us, 267 where both share the loops */
 #pragma unroll
     for (int u = 0; u < NORM_PACKS; ++u) v[u] = __builtin_nontemporal_load(reinterpret_cast<const VL*>(src + piece.at(u)));
-  } else {
+    if (!factor_of(factor)) return;
 #pragma unroll
-    for (int u = 0; u < NORM_PACKS; ++u) v[u] = piece.template cut<W>(src, u);
+    for (int u = 0; u < NORM_PACKS; ++u) {
+      P out[W];
+      scaled(u, out);
+      store_pack_nt_loose<T, W>(dst + piece.at(u), out);
+    }
+    return;
   }
-  double total;
-  if constexpr (FUSED) {
-    __shared__ double slots[NORM_THREADS / WAVE];
-    total = ::sqrt(norm_of(norm_in, partials, slots));
-    if (blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = total;
-  } else {
-    total = norm_in[0];
-  }
-  const bool within = total <= max_norm;
-  if (src == dst && within) return; /* nothing to do in place */
-  const P factor = within ? (P)1 : (P)(max_norm / total);
+#pragma unroll
+  for (int u = 0; u < NORM_PACKS; ++u) v[u] = piece.template cut<W>(src, u);
+  if (!factor_of(factor)) return;
 #pragma unroll
   for (int u = 0; u < NORM_PACKS; ++u) {
     const size_t i = piece.at(u);
     P out[W];
-#pragma unroll
-    for (int j = 0; j < W; ++j) out[j] = (P)v[u][j] * factor;
-    if (whole || i + W <= piece.left) {
+    scaled(u, out);
+    if (i + W <= piece.left) {
       store_pack_nt_loose<T, W>(dst + i, out);
     } else {
 #pragma unroll
