@@ -238,3 +238,23 @@ def test_no_token_scales_the_gradient(dtype, n):
         G._call("embedding_i_ij_reverse", dtype, none.data_ptr(), None, dt.t.data_ptr(), None, 2.0, alpha, 8, v, 0, n)
         assert torch.equal(dt.t.cpu(), (old.double() * alpha).to(dtype)), f"{dtype} n={n} alpha={alpha}"
         dt.check(f"no token {dtype} n={n} alpha={alpha}")
+
+
+@pytest.mark.parametrize("m", [300, 9000])
+def test_many_tokens_and_rows_beyond_32_bit_offsets(m):
+    """As above, by both ways of ordering the tokens; named rows sit at both ends of the table."""
+    v, n = 140000, 32768
+    g = torch.full((v, n), 7.0, dtype=F16, device="cuda")
+    tokens = torch.cat([torch.arange(m // 2), torch.arange(v - m // 3, v), torch.full((m - m // 2 - m // 3,), -1)])
+    tokens = tokens[torch.randperm(m, generator=gen(4))].cuda()
+    dy = torch.randn(m, n, device="cuda", dtype=torch.float32).to(F16)
+    sc = scratch_for(F16, v, m, n)
+    G.say(f"lookup reverse of {m} tokens, a table past 2^32 elements")
+    lookup_reverse(tokens, dy, g, sc.t, 0.5)
+    torch.cuda.synchronize()
+    sc.check("scratch")
+    order = torch.argsort(tokens)
+    live = order[tokens[order] >= 0]  # every id once: halving is exact (or rounds as the plain form does)
+    assert torch.equal(g[tokens[live]], dy[live] * 0.5)
+    g[tokens[live]] = 0
+    assert not bool(g.any())

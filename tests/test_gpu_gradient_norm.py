@@ -187,3 +187,34 @@ def test_results_do_not_change_from_run_to_run(dtype):
         got = [norm, *outs]
         first = first or got
         assert all(torch.equal(x, y) for x, y in zip(got, first))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("count", [119, 120, 121, 122, 240, 241, 242])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_numbers_of_runs(dtype, count, in_place):
+    """Tensors apart from each other, around one and two launches' arguments."""
+    check(dtype, [(37 * k) % 1000 + 1 for k in range(count)], 2.0, f"{dtype} {count} runs in place {in_place}", in_place, shift=1)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_pieces_that_the_last_launch_adds_up_or_not(dtype):
+    """Around 2048 pieces of 16 KiB, and a last piece that ends in a pack, behind one and in the middle of one."""
+    each = 16384 // dtype.itemsize
+    for pieces in (2047, 2048, 2049):
+        for less in (0, 1, each - 1, each // 2):
+            check(dtype, [pieces * each - less], 3.0, f"{dtype} {pieces} pieces less {less} elements", in_place=True)
+
+
+def test_a_tensor_of_more_than_2_32_elements():
+    k = 2 ** 32 + 12345
+    t, small = torch.zeros(k, dtype=F16, device="cuda"), torch.full((5,), 2.0, dtype=F16, device="cuda")
+    where = torch.tensor([0, 2 ** 31 + 1, 2 ** 32 - 1, 2 ** 32, k - 1], device="cuda")
+    t[where] = 4.0
+    norm = a_norm()
+    G.say("clip a tensor of more than 2^32 elements")
+    clip([t, small], [t, small], F16, norm, 5.0)
+    assert float(norm) == 10.0  # 5 * 16 + 5 * 4 under the root
+    assert torch.equal(t[where], torch.full((5,), 2.0, dtype=F16, device="cuda")) and bool((small == 1.0).all())
+    t[where] = 0
+    assert not bool(t.any())

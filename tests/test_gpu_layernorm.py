@@ -257,3 +257,40 @@ def test_the_gradient_agrees_with_differences():
             up[k], down[k] = t + step * way, t - step * way
             slope = (value(*up) - value(*down)) / (2 * step)
             assert abs(slope - float((grad * way).sum())) < 1e-7 * max(1.0, abs(slope))
+
+
+def test_rows_beyond_32_bit_offsets():
+    """Operands of more than 2^32 elements, with values in their first and last rows."""
+    m, n, k = 140000, 32768, 3
+    part = torch.cat([torch.arange(k), torch.arange(m - k, m)])
+    xs, ds, gain, bias = normal((2 * k, n), F16, 1), normal((2 * k, n), F16, 2), normal((n,), F16, 3), normal((n,), F16, 4)
+    x, other = torch.zeros(m, n, dtype=F16, device="cuda"), torch.full((m, n), 9.0, dtype=F16, device="cuda")
+    x[part] = xs.cuda()
+    G.say("layernorm forward past 2^32 elements")
+    forward(x, gain.cuda(), bias.cuda(), other)
+    torch.cuda.synchronize()
+    P.close(other[part], *P.layernorm(xs, gain, bias, EPS, F16), "layernorm past 2^32 elements")
+    assert torch.equal(other[k:m - k:997].cpu(), bias.expand(len(range(k, m - k, 997)), n))  # rows of zeros
+    other.zero_()
+    other[part] = ds.cuda()
+    dg, db, sc = torch.empty(n, dtype=F16, device="cuda"), torch.empty(n, dtype=F16, device="cuda"), scratch_for(F16, m, n)
+    G.say("layernorm reverse past 2^32 elements")
+    reverse(x, gain.cuda(), other, other, dg, db, sc.t)
+    torch.cuda.synchronize()
+    sc.check("scratch")
+    refs, bounds = P.layernorm_reverse(xs, gain, ds, EPS, F16)  # rows without a gradient add nothing
+    for name, got, ref, bound in zip(("dx", "dg", "db"), (other[part], dg, db), refs, bounds):
+        P.close(got, ref, bound, f"{name} past 2^32 elements")
+    assert not bool(other[k:m - k].any())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n", [(1, 4096), (2, 4096), (4, 4096), (5, 4096), (16, 512), (32, 512), (33, 512), (64, 256), (65, 256), (130, 128), (257, 64), (4, 20000)])
+def test_few_rows(dtype, m, n):
+    """Around what one workgroup takes, which writes the vectors' gradients by itself."""
+    x, dy, gain = normal((m, n), dtype, 1), normal((m, n), dtype, 2), normal((n,), dtype, 3)
+    for alpha in (0.0, 0.5):
+        check_reverse(x, gain, dy, f"{dtype} few rows {m}x{n} alpha {alpha}", alpha=alpha)
+        check_reverse(x, gain, dy, f"{dtype} few rows {m}x{n} alpha {alpha}, off alignment", shifts=(1, 0, 0, 1, 1), alpha=alpha)
+    check_reverse(x, gain, dy, f"{dtype} few rows {m}x{n}, no bias", want=(True, False))
+    check_reverse(x, None, dy, f"{dtype} few rows {m}x{n}, no gain", want=(False, True), in_place=True)
