@@ -294,3 +294,25 @@ def test_few_rows(dtype, m, n):
         check_reverse(x, gain, dy, f"{dtype} few rows {m}x{n} alpha {alpha}, off alignment", shifts=(1, 0, 0, 1, 1), alpha=alpha)
     check_reverse(x, gain, dy, f"{dtype} few rows {m}x{n}, no bias", want=(True, False))
     check_reverse(x, None, dy, f"{dtype} few rows {m}x{n}, no gain", want=(False, True), in_place=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n", [(7, 9), (5000, 24), (3000, 200), (3001, 1027), (2500, 2048), (1500, 5121), (600, 12288), (5, 40961)])
+@pytest.mark.parametrize("alpha", [0.0, 0.5])
+def test_many_rows_in_place(dtype, m, n, alpha):
+    """Workgroups that walk several rows, with the next ones on their way while these are written: over dy, and over x."""
+    x, gain, bias, dy = normal((m, n), dtype, 1), normal((n,), dtype, 2, 0.2, 1.0), normal((n,), dtype, 3), normal((m, n), dtype, 4)
+    if alpha == 0.0:
+        check_forward(x, gain, bias, f"{dtype} [{m},{n}] in place", in_place=True)
+    check_reverse(x, gain, dy, f"{dtype} [{m},{n}] dx over dy alpha {alpha}", in_place=True, alpha=alpha)
+    what = f"{dtype} [{m},{n}] dx over x alpha {alpha}"
+    X, D, old = guarded(x), guarded(dy), [x, normal((n,), dtype, 5), normal((n,), dtype, 6)]
+    dg, db, sc = guarded(old[1]), guarded(old[2]), scratch_for(dtype, m, n)
+    G.say(f"layernorm reverse {what}")
+    reverse(X.t, gain.cuda(), D.t, X.t, dg.t, db.t, sc.t, alpha=alpha)
+    torch.cuda.synchronize()
+    for k in (X, D, dg, db, sc):
+        k.check(what)
+    refs, bounds = P.layernorm_reverse(x, gain, dy, EPS, dtype, alpha, old)
+    for name, got, ref, bound in zip(("dx", "dg", "db"), (X, dg, db), refs, bounds):
+        P.close(got.t, ref, bound, f"layernorm {name} {what}")

@@ -151,6 +151,30 @@ def test_on_a_side_stream_of_torch():
     s.check("side stream")
 
 
+@pytest.mark.parametrize("m,n", [(1, 4096), (30, 200), (256, 96), (3, 20000)])
+def test_replays_of_a_captured_short_batch(m, n):
+    s = Step(F16, 700, m, n, 6)
+    s.enqueue(G._call)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    G.say(f"capture of a short batch {m}x{n}")
+    with torch.cuda.graph(graph):
+        s.enqueue(G._call)
+    for replay in range(4):
+        s.tokens.copy_((s.tokens + replay * 37) % 700)
+        s.dp.mul_(-0.5)
+        for t in s.results():
+            t.fill_(float("nan"))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in s.results()]
+        s.enqueue(G._call)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, s.results())), f"replay {replay}"
+    s.check("after the replays")
+
+
 def _load(d, name, shape, dtype=np.float32):
     return torch.from_numpy(np.fromfile(os.path.join(d, name + ".bin"), dtype=dtype).reshape(shape))
 
