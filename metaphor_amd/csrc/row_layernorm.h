@@ -704,9 +704,12 @@ __global__ __launch_bounds__(BLOCK) void layernorm_rev_rows(
 
 /* ------------------------------------------------------------------ dg and db from the partial rows */
 
-/* The partial rows added in a fixed order in fp64. A workgroup owns a 128-byte line of columns; its 64 slices
- * take the rows in turn, a 16-byte load of eight rows on its way at once. */
-constexpr int NORM_FINISH_LANES = 8, NORM_FINISH_SLICES = 64;
+/* The partial rows added in a fixed order in fp64. A workgroup owns a 128-byte line of columns; its 32 slices
+ * take the rows in turn, a 16-byte load of eight rows on its way at once. Bound by the latency of a launch that
+ * waits for the one before it: 4 us behind the row pass (r32 [8192, 4096], 256 partial rows; 64 slices 0.5 us
+ * more, 128 1.7 more, 16 0.3; at 100 partial rows of r16 [100, 12288] the whole reverse 14.3 us at 32 slices,
+ * 15.7 at 64, 13.8 at 16). */
+constexpr int NORM_FINISH_LANES = 8, NORM_FINISH_SLICES = 32;
 template <class T>
 __global__ __launch_bounds__(NORM_FINISH_LANES * NORM_FINISH_SLICES) void layernorm_grads_finish(
     const typename precision<T>::type* partials, T* dg, T* db, double alpha, int rows, size_t n) {
