@@ -290,7 +290,8 @@ __global__ __launch_bounds__(SORT_THREADS) void embedding_sort_place(
 
 /* ------------------------------------------------------------------ sums over the sorted places */
 
-/* The first of the sorted keys that is at least `key`, m if there is none. */
+/* The first of the sorted keys that is at least `key`, m if there is none. (Seven probes a step are fewer steps
+ * and more loads: r16 65536 places, 151936 x 2048, 189 us for 183.) */
 __device__ __forceinline__ size_t lower_bound(const unsigned* keys, size_t m, unsigned key) {
   size_t lo = 0, hi = m;
   while (lo < hi) {
@@ -311,28 +312,28 @@ inline unsigned embedding_fill_rows(size_t row_bytes) {
   return rows < 1 ? 1 : rows < FILL_MOST ? (unsigned)rows : FILL_MOST;
 }
 
-/* The places of one id, a run of equal keys, around entry i, as far as `reach` entries before and behind it:
- * [begin, end). */
-struct Run { size_t begin, end; };
-__device__ __forceinline__ Run run_around(const unsigned* keys, size_t m, size_t i, size_t reach) {
-  const unsigned key = keys[i];
-  size_t lo = i > reach ? i - reach : 0, hi = i; /* the first equal one lies in [lo, hi] */
-  while (lo < hi) {
-    const size_t mid = (lo + hi) / 2;
-    if (keys[mid] < key) lo = mid + 1;
-    else hi = mid;
-  }
-  Run r;
-  r.begin = lo;
-  lo = i + 1; /* the first greater one in [lo, hi] */
-  hi = i + reach < m ? i + reach : m;
-  while (lo < hi) {
-    const size_t mid = (lo + hi) / 2;
-    if (keys[mid] == key) lo = mid + 1;
-    else hi = mid;
-  }
-  r.end = lo;
-  return r;
+/* What happens at a boundary between chunks, entry i: `cut`: an id's places (a run of equal keys) lie on both
+ * sides; then `after` of them from i on, and `over`: there are more than a chunk of them. A lane each looks at
+ * a chunk's entries before the boundary and a chunk's behind it, so votes say all of it after one load; binary
+ * searches are a dozen loads, one behind the other (the whole gradient, r32 3965 places of 114 rows of 1280:
+ * 26.4 us, with votes 22.7; 8192 of 50257 x 1024 added to what is there 31.1 and 29.8). All lanes of the wavefront call it with the same i. */
+struct ChunkEdge {
+  bool cut, over;
+  unsigned after;
+};
+__device__ __forceinline__ unsigned edge_key(const unsigned* keys, size_t m, size_t i, unsigned chunk) {
+  const unsigned l = threadIdx.x % WAVE;
+  const size_t at = i - chunk + l;
+  return i > 0 && i < m && l < 2 * chunk && at < m ? keys[at] : 0xffffffffu; /* no id's key */
+}
+__device__ __forceinline__ ChunkEdge chunk_edge(unsigned key, size_t m, size_t i, unsigned chunk) {
+  const unsigned long long same = __ballot(key == (unsigned)__builtin_amdgcn_readlane((int)key, (int)chunk));
+  const unsigned before = (unsigned)__builtin_clzll(~(same << (WAVE - chunk))); /* up to chunk of them: zeros come in below */
+  ChunkEdge e;
+  e.after = (unsigned)__builtin_ctzll(~(same >> chunk)); /* likewise */
+  e.cut = i > 0 && i < m && before > 0;
+  e.over = before + e.after > chunk;
+  return e;
 }
 
 /* Rows [row0, row0 + rows) of the table but those that are named: cleared, or (BLEND) scaled. */
@@ -394,21 +395,27 @@ __global__ __launch_bounds__(256) void embedding_sum(
   const int sub = threadIdx.x / G, lane = threadIdx.x % G;
   const size_t c = (size_t)(blockIdx.x / strips) * (256 / G) + sub;
   const int p = (int)(blockIdx.x % strips) * G + lane;
-  size_t lo = c * chunk;
-  if (lo >= m || p >= rp.npk) return;
-  size_t hi = lo + chunk < m ? lo + chunk : m;
-  bool begun = false, goes_on = false; /* the first id began, the last one goes on in another chunk */
-  if (hi < m && keys[hi - 1] == keys[hi]) {
-    const Run r = run_around(keys, m, hi, chunk + 1);
-    goes_on = r.end - r.begin > chunk;
-    if (!goes_on) hi = r.end;
+  size_t lo = c * chunk, hi = lo + chunk < m ? lo + chunk : m;
+  bool begun = false, goes_on = false; /* the first id began in another chunk, the last one goes on in another */
+  constexpr int NG = G < WAVE ? WAVE / G : 1; /* chunks a wavefront */
+  const size_t first = G < WAVE ? (size_t)blockIdx.x / strips * (256 / G) + threadIdx.x / WAVE * NG : c;
+  unsigned at_edge[NG + 1];
+#pragma unroll
+  for (int g = 0; g <= NG; ++g) at_edge[g] = edge_key(keys, m, (first + g) * chunk, (unsigned)chunk);
+#pragma unroll
+  for (int g = 0; g <= NG; ++g) {
+    const size_t i = (first + g) * chunk;
+    const ChunkEdge e = chunk_edge(at_edge[g], m, i, (unsigned)chunk);
+    if (!e.cut) continue;
+    if (first + g == c) {
+      begun = e.over;
+      if (!e.over) lo = i + e.after;
+    } else if (first + g == c + 1) {
+      goes_on = e.over;
+      if (!e.over) hi = i + e.after;
+    }
   }
-  if (lo > 0 && keys[lo - 1] == keys[lo]) {
-    const Run r = run_around(keys, m, lo, chunk + 1);
-    begun = r.end - r.begin > chunk;
-    if (!begun) lo = r.end;
-  }
-  if (lo >= hi) return;
+  if (lo >= hi || p >= rp.npk) return;
 
   P acc[W];
   unsigned current = keys[lo];
@@ -563,9 +570,10 @@ __global__ __launch_bounds__(256) void embedding_direct(
 }
 
 /* The ids that cross chunks: the partial rows of each are added up in order, in fp64. Workgroups take (id,
- * strip of JOIN_LANES * CW columns) in turn; the slices of a workgroup take the partial rows in turn, four
- * on their way, and are then added. */
-constexpr int JOIN_LANES = 32, JOIN_SLICES = 256 / JOIN_LANES;
+ * strip of JOIN_LANES * CW columns) in turn; the slices of a workgroup take the partial rows in turn, eight
+ * on their way, and are then added (r16 22002 places of 383 rows of 128: 30 us; 35 with four on their way and
+ * 256 chunks looked at together). */
+constexpr int JOIN_LANES = 32, JOIN_SLICES = 256 / JOIN_LANES, JOIN_LOOKS = 4, JOIN_ROWS = 8;
 template <class T, int CW, bool BLEND>
 __global__ __launch_bounds__(256) void embedding_join(
     const unsigned* keys, const typename precision<T>::type* partials, const unsigned* crossing, const unsigned* list, T* grads,
@@ -579,34 +587,38 @@ __global__ __launch_bounds__(256) void embedding_join(
   for (unsigned q = blockIdx.x; q < work; q += gridDim.x) {
     const size_t c = list[q / strips];
     const unsigned key = keys[(c + 1) * chunk - 1]; /* the id that goes on in the chunk behind */
-    /* the chunks behind c that begin with the id: 256 at a time */
+    /* the chunks behind c that begin with the id, 1024 at a time: sorted, so they are the first ones */
     size_t later = 0;
     for (;;) {
-      const size_t at = (c + 1 + later + threadIdx.x) * chunk;
-      const unsigned long long same = __ballot(at < m && keys[at] == key);
-      if (threadIdx.x % WAVE == 0) ends[threadIdx.x / WAVE] = (unsigned)__builtin_popcountll(same); /* sorted: the first ones */
+      unsigned same = 0;
+#pragma unroll
+      for (int k = 0; k < JOIN_LOOKS; ++k) {
+        const size_t at = (c + 1 + later + k * 256 + threadIdx.x) * chunk;
+        same += (unsigned)__builtin_popcountll(__ballot(at < m && keys[at < m ? at : 0] == key));
+      }
+      if (threadIdx.x % WAVE == 0) ends[threadIdx.x / WAVE] = same;
       __syncthreads();
       unsigned found = 0;
 #pragma unroll
       for (int w = 0; w < 256 / WAVE; ++w) found += ends[w];
       later += found;
       __syncthreads();
-      if (found < 256) break;
+      if (found < JOIN_LOOKS * 256) break;
     }
     const size_t j = (size_t)(q % strips) * COLS + l * CW;
     double s[CW];
 #pragma unroll
     for (int i = 0; i < CW; ++i) s[i] = 0.0;
     if (j < n) { /* CW > 1: n is a multiple of it */
-      for (size_t k0 = slice; k0 <= later; k0 += 4 * JOIN_SLICES) {
-        P t[4][CW];
+      for (size_t k0 = slice; k0 <= later; k0 += JOIN_ROWS * JOIN_SLICES) {
+        P t[JOIN_ROWS][CW];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < JOIN_ROWS; ++u) {
           const size_t k = k0 + u * JOIN_SLICES <= later ? k0 + u * JOIN_SLICES : k0;
           load_pack_nt<P, CW>(partials + ((c + k) * 2 + (k == 0 ? 1 : 0)) * n + j, t[u]);
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < JOIN_ROWS; ++u)
 #pragma unroll
           for (int i = 0; i < CW; ++i) s[i] += k0 + u * JOIN_SLICES <= later ? (double)t[u][i] : 0.0;
       }
