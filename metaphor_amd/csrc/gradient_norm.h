@@ -8,11 +8,12 @@
  * double on the device; nothing waits for the host.
  *
  * Tensors that lie one behind the other (a bucket of gradients) are walked as one run. The runs' addresses
- * and sizes travel as kernel arguments, NORM_RUNS of them a launch: nothing is copied to the device and a
+ * and sizes travel as kernel arguments, up to 196 of them a launch: nothing is copied to the device and a
  * captured launch keeps its own table. A table's work is cut into pieces of NORM_PIECE bytes, four 16-byte
  * packs a thread; workgroups take them in turn for the squares, each leaving one partial sum in the
- * workspace, and one each for the scaling (1024 workgroups for the squares: 203 M elements in 400 tensors 419 us
- * to clip, 2048 425, 100 tensors of 1000 elements the norm 6.4 and 7.0).
+ * workspace, and one each for the scaling (1024 workgroups for the squares: 100 tensors of 1000 elements the
+ * norm 6.4 us, by 2048 7.0, and 203 M elements in 400 tensors 148 and 154; 196 runs a launch rather than 120
+ * make the 148 137).
  *
  * The squares are bound by reading the tensors once, the scaling by reading and writing them once. r32,
  * 203 M elements: squares 124 us (6.6 TB/s), both together 367 us, of which the scaling on its own would
@@ -32,7 +33,7 @@
 
 namespace mp {
 
-constexpr int NORM_RUNS = 120, NORM_THREADS = 256, NORM_PACKS = 4;
+constexpr int NORM_THREADS = 256, NORM_PACKS = 4;
 constexpr size_t NORM_PIECE = (size_t)NORM_THREADS * NORM_PACKS * PACK_BYTES, NORM_PARTIALS = 1024; /* a table */
 /* up to so many pieces the scaling adds up the partial sums itself, in every workgroup, and one launch is
  * saved; beyond, a workgroup would spend as long on that as on its piece */
@@ -40,18 +41,22 @@ constexpr size_t NORM_FUSED_PIECES = 2048;
 
 constexpr size_t NORM_KEPT_BYTES = (size_t)224 << 20, NORM_KEPT_PIECES = NORM_KEPT_BYTES / NORM_PIECE;
 
-template <class T> struct NormTable {
-  const T* src[NORM_RUNS];
-  T* dst[NORM_RUNS];
-  unsigned long long size[NORM_RUNS];
-  unsigned first[NORM_RUNS + 1]; /* the number of the run's first piece; [count] is the end */
+/* Runs of a launch: as many as 4 KiB of arguments hold. APART: the results lie elsewhere. */
+constexpr int norm_runs(bool apart) { return apart ? 140 : 196; }
+template <class T, bool APART> struct NormTable {
+  static constexpr int RUNS = norm_runs(APART);
+  const T* src[RUNS];
+  T* dst[APART ? RUNS : 1];
+  unsigned long long size[RUNS];
+  unsigned first[RUNS + 1]; /* the number of the run's first piece; [count] is the end */
   int count;
 };
+static_assert(sizeof(NormTable<r16, true>) <= 4032 && sizeof(NormTable<r16, false>) <= 4032, "room for the other arguments");
 
 /* The run that piece `q` belongs to: the last one whose first piece is not behind it (runs have a piece at
  * least). Scalar loads from the argument block; one vector load a wavefront and a vote cost the scaling
  * of 100 runs 3 %. */
-template <class T> __device__ __forceinline__ int norm_run_of(const NormTable<T>& t, unsigned q) {
+template <class TABLE> __device__ __forceinline__ int norm_run_of(const TABLE& t, unsigned q) {
   int lo = 0, hi = t.count - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) / 2;
@@ -67,7 +72,7 @@ template <class T> struct NormPiece {
   static constexpr size_t LEN = NORM_PIECE / sizeof(T);
   int run;
   size_t lo, left; /* the piece's first element in its run, and the run's elements from there on */
-  __device__ __forceinline__ NormPiece(const NormTable<T>& t, unsigned q) {
+  template <class TABLE> __device__ __forceinline__ NormPiece(const TABLE& t, unsigned q) {
     run = norm_run_of(t, q);
     lo = (size_t)(q - t.first[run]) * LEN;
     left = t.size[run] - lo;
@@ -96,7 +101,7 @@ __device__ __forceinline__ double norm_block_sum(double s, double* slots) {
   return t;
 }
 
-template <bool KEEP, class T> __device__ __forceinline__ double piece_squares(const NormTable<T>& t, unsigned q) {
+template <bool KEEP, class T> __device__ __forceinline__ double piece_squares(const NormTable<T, false>& t, unsigned q) {
   constexpr int W = NormPiece<T>::W;
   using VL = typename loose_vec_of<T, W>::type;
   const NormPiece<T> piece(t, q);
@@ -126,7 +131,7 @@ template <bool KEEP, class T> __device__ __forceinline__ double piece_squares(co
 }
 
 /* Pieces from `keep` on through loads that leave them in the memory-side cache. */
-template <class T> __global__ __launch_bounds__(NORM_THREADS) void gradient_squares(NormTable<T> t, unsigned keep, double* partials) {
+template <class T> __global__ __launch_bounds__(NORM_THREADS) void gradient_squares(NormTable<T, false> t, unsigned keep, double* partials) {
   __shared__ double slots[NORM_THREADS / WAVE];
   const unsigned end = t.first[t.count];
   double s = 0.0;
@@ -154,14 +159,14 @@ static __global__ __launch_bounds__(NORM_THREADS) void gradient_norm_finish(cons
 }
 
 /* FUSED: norm_in is what the squares left, `partials` sums; the first workgroup writes the norm. */
-template <class T, bool FUSED>
-__global__ __launch_bounds__(NORM_THREADS) void gradient_scaled(NormTable<T> t, const double* norm_in, unsigned partials, double* norm_out, double max_norm) {
+template <class T, bool FUSED, bool APART>
+__global__ __launch_bounds__(NORM_THREADS) void gradient_scaled(NormTable<T, APART> t, const double* norm_in, unsigned partials, double* norm_out, double max_norm) {
   using P = typename precision<T>::type;
   constexpr int W = NormPiece<T>::W;
   using VL = typename loose_vec_of<T, W>::type;
   const NormPiece<T> piece(t, blockIdx.x);
   const T* src = t.src[piece.run] + piece.lo;
-  T* dst = t.dst[piece.run] + piece.lo;
+  T* dst = APART ? t.dst[piece.run] + piece.lo : const_cast<T*>(src);
   /* what to scale by; false: nothing to do in place */
   auto factor_of = [&](P& factor) {
     double total;
@@ -234,6 +239,13 @@ template <class T, class F> inline void for_norm_runs(const void* const* grads, 
   }
 }
 
+/* whether any result lies elsewhere than its gradient */
+inline bool gradients_apart(const void* const* grads, const void* const* outs, const len_t* sizes, size_t count) {
+  for (size_t k = 0; k < count; ++k)
+    if (sizes[k] && grads[k] != outs[k]) return true;
+  return false;
+}
+
 struct NormWork { size_t runs, pieces; };
 template <class T> inline NormWork norm_work(const void* const* grads, const void* const* outs, const len_t* sizes, size_t count) {
   NormWork w{0, 0};
@@ -244,19 +256,19 @@ template <class T> inline NormWork norm_work(const void* const* grads, const voi
   return w;
 }
 
-/* f(table) for the runs in groups of NORM_RUNS */
-template <class T, class F>
+/* f(table) for the runs in groups of a table's */
+template <class T, bool APART, class F>
 inline void for_norm_tables(const void* const* grads, const void* const* outs, const len_t* sizes, size_t count, F&& f) {
-  NormTable<T> t;
+  NormTable<T, APART> t;
   t.count = 0;
   t.first[0] = 0;
-  for_norm_runs<T>(grads, outs, sizes, count, [&](size_t k, size_t size) {
+  for_norm_runs<T>(grads, APART ? outs : nullptr, sizes, count, [&](size_t k, size_t size) {
     t.src[t.count] = static_cast<const T*>(grads[k]);
-    t.dst[t.count] = outs ? const_cast<T*>(static_cast<const T*>(outs[k])) : nullptr;
+    if constexpr (APART) t.dst[t.count] = const_cast<T*>(static_cast<const T*>(outs[k]));
     t.size[t.count] = size;
     const size_t pieces = (size * sizeof(T) + NORM_PIECE - 1) / NORM_PIECE;
     t.first[t.count + 1] = t.first[t.count] + (unsigned)pieces;
-    if (++t.count == NORM_RUNS) {
+    if (++t.count == norm_runs(APART)) {
       f(t);
       t.count = 0;
     }
@@ -266,7 +278,7 @@ inline void for_norm_tables(const void* const* grads, const void* const* outs, c
 
 /* Every table leaves at most NORM_PARTIALS sums. Tensors that form runs make fewer tables than they might,
  * never more. */
-inline size_t gradient_norm_scratch_bytes(size_t count) { return (count + NORM_RUNS - 1) / NORM_RUNS * NORM_PARTIALS * sizeof(double); }
+inline size_t gradient_norm_scratch_bytes(size_t count) { return (count + norm_runs(false) - 1) / norm_runs(false) * NORM_PARTIALS * sizeof(double); }
 
 /* Every argument, before the first launch. outs NULL where none are written. */
 template <class T>
@@ -333,7 +345,7 @@ template <class T> inline void gradient_check_apart(const void* const* grads, co
 template <class T>
 inline unsigned gradient_squares_all(const void* const* grads, const len_t* sizes, double* partials, size_t count, hipStream_t stream) {
   unsigned used = 0;
-  for_norm_tables<T>(grads, nullptr, sizes, count, [&](const NormTable<T>& t) {
+  for_norm_tables<T, false>(grads, nullptr, sizes, count, [&](const NormTable<T, false>& t) {
     const unsigned pieces = t.first[t.count], blocks = pieces < NORM_PARTIALS ? pieces : (unsigned)NORM_PARTIALS;
     const unsigned keep = pieces > NORM_KEPT_PIECES ? pieces - (unsigned)NORM_KEPT_PIECES : 0;
     gradient_squares<T><<<dim3(blocks), dim3(NORM_THREADS), 0, stream>>>(t, keep, partials + used);
@@ -346,12 +358,16 @@ inline unsigned gradient_squares_all(const void* const* grads, const len_t* size
 template <class T>
 inline void gradient_scale_all(const void* const* grads, const void* const* outs, const len_t* sizes, const double* norm_in, unsigned partials, double* norm_out,
                                double max_norm, size_t count, hipStream_t stream) {
-  for_norm_tables<T>(grads, outs, sizes, count, [&](const NormTable<T>& t) {
-    const dim3 grid(t.first[t.count]), block(NORM_THREADS);
-    if (norm_out) gradient_scaled<T, true><<<grid, block, 0, stream>>>(t, norm_in, partials, norm_out, max_norm);
-    else gradient_scaled<T, false><<<grid, block, 0, stream>>>(t, norm_in, 0, nullptr, max_norm);
-    MP_CHECK_LAUNCH();
-  });
+  auto as = [&]<bool APART>() {
+    for_norm_tables<T, APART>(grads, outs, sizes, count, [&](const NormTable<T, APART>& t) {
+      const dim3 grid(t.first[t.count]), block(NORM_THREADS);
+      if (norm_out) gradient_scaled<T, true, APART><<<grid, block, 0, stream>>>(t, norm_in, partials, norm_out, max_norm);
+      else gradient_scaled<T, false, APART><<<grid, block, 0, stream>>>(t, norm_in, 0, nullptr, max_norm);
+      MP_CHECK_LAUNCH();
+    });
+  };
+  if (gradients_apart(grads, outs, sizes, count)) as.template operator()<true>();
+  else as.template operator()<false>();
 }
 
 template <class T>
@@ -386,7 +402,7 @@ inline void gradient_clip(const void* grads, const void* outs, const void* sizes
   double *partials = static_cast<double*>(scratch), *out = static_cast<double*>(norm);
   const unsigned used = gradient_squares_all<T>(src, lengths, partials, count, stream);
   const NormWork work = norm_work<T>(src, dst, lengths, count);
-  const bool fused = used > 0 && work.runs <= (size_t)NORM_RUNS && work.pieces <= NORM_FUSED_PIECES;
+  const bool fused = used > 0 && work.runs <= (size_t)norm_runs(gradients_apart(src, dst, lengths, count)) && work.pieces <= NORM_FUSED_PIECES;
   if (!fused) {
     gradient_norm_finish<<<dim3(1), dim3(NORM_THREADS), 0, stream>>>(partials, used, 0.0, out);
     MP_CHECK_LAUNCH();

@@ -198,6 +198,26 @@ def test_numbers_of_runs(dtype, count, in_place):
 
 
 @pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("count", [139, 140, 141, 195, 196, 197, 280, 281, 392, 393])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_more_numbers_of_runs(dtype, count, in_place):
+    """The same where results of their own take room among the arguments, and where none do."""
+    check(dtype, [(37 * k) % 300 + 1 for k in range(count)], 2.0, f"{dtype} {count} runs in place {in_place}", in_place, shift=1)
+
+
+def test_some_results_in_place_and_some_apart():
+    plain = [normal((300 + k,), F32, k) for k in range(9)]
+    src, norm = [guarded(t) for t in plain], a_norm()
+    out = [s if k % 3 else G.Guarded((300 + k,), F32, 1, fill=float("nan")) for k, s in enumerate(src)]
+    clip([s.t for s in src], [o.t for o in out], F32, norm, 1.0)
+    ref, _ = P.gradient_norm(plain)
+    for k, (p, s, o) in enumerate(zip(plain, src, out)):
+        s.check(f"gradient {k}"), o.check(f"result {k}")
+        P.close(o.t, *P.clipped(p, ref, 1.0, F32), f"clipped {k}")
+        assert k % 3 or torch.equal(s.t.cpu(), p)
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
 def test_pieces_that_the_last_launch_adds_up_or_not(dtype):
     """Around 2048 pieces of 16 KiB, and a last piece that ends in a pack, behind one and in the middle of one."""
     each = 16384 // dtype.itemsize
