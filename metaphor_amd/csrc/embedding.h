@@ -16,7 +16,7 @@
  * alpha = 0 the sort's launches, which use a fraction of the GPU, clear the table's first rows on the
  * way, named or not. All of it is bound by memory: dy read once, the table written once. r32 8192 places,
  * 50257 rows of 1024: 54 us (4.3 TB/s, of which the ordering is 13 us and the join 5); r16 65536 places,
- * 151936 rows of 2048: 182 us (4.9 TB/s; the sums' launch 144 us). The lookup, r32 16384 places of rows of 2048:
+ * 151936 rows of 2048: 176 us (5.1 TB/s; the sums' launch 135 us). The lookup, r32 16384 places of rows of 2048:
  * 31 us (6.2 TB/s).
  */
 #ifndef MP_EMBEDDING_H
@@ -570,10 +570,11 @@ __global__ __launch_bounds__(256) void embedding_direct(
 }
 
 /* The ids that cross chunks: the partial rows of each are added up in order, in fp64. Workgroups take (id,
- * strip of JOIN_LANES * CW columns) in turn; the slices of a workgroup take the partial rows in turn, eight
- * on their way, and are then added (r16 22002 places of 383 rows of 128: 30 us; 35 with four on their way and
- * 256 chunks looked at together). */
-constexpr int JOIN_LANES = 32, JOIN_SLICES = 256 / JOIN_LANES, JOIN_LOOKS = 4, JOIN_ROWS = 8;
+ * strip of JOIN_LANES * CW columns) in turn; the slices of a workgroup take the partial rows in turn, up
+ * to eight on their way, and are then added. One, four and eight of them by how many there are (always four:
+ * r16 22002 places of 383 rows of 128 take 35.6 us for 31.1; always eight: 65536 of 151936 x 2048 178 for 176);
+ * the chunks an id reaches are looked for among 256 first, then 1024 at a time (always 1024: 183). */
+constexpr int JOIN_LANES = 32, JOIN_SLICES = 256 / JOIN_LANES, JOIN_LOOKS = 4;
 template <class T, int CW, bool BLEND>
 __global__ __launch_bounds__(256) void embedding_join(
     const unsigned* keys, const typename precision<T>::type* partials, const unsigned* crossing, const unsigned* list, T* grads,
@@ -587,14 +588,15 @@ __global__ __launch_bounds__(256) void embedding_join(
   for (unsigned q = blockIdx.x; q < work; q += gridDim.x) {
     const size_t c = list[q / strips];
     const unsigned key = keys[(c + 1) * chunk - 1]; /* the id that goes on in the chunk behind */
-    /* the chunks behind c that begin with the id, 1024 at a time: sorted, so they are the first ones */
+    /* the chunks behind c that begin with the id: sorted, so they are the first ones */
     size_t later = 0;
-    for (;;) {
+    for (int looks = 1;; looks = JOIN_LOOKS) {
       unsigned same = 0;
 #pragma unroll
       for (int k = 0; k < JOIN_LOOKS; ++k) {
         const size_t at = (c + 1 + later + k * 256 + threadIdx.x) * chunk;
-        same += (unsigned)__builtin_popcountll(__ballot(at < m && keys[at < m ? at : 0] == key));
+        const bool look = k < looks && at < m;
+        same += (unsigned)__builtin_popcountll(__ballot(look && keys[look ? at : 0] == key));
       }
       if (threadIdx.x % WAVE == 0) ends[threadIdx.x / WAVE] = same;
       __syncthreads();
@@ -603,25 +605,30 @@ __global__ __launch_bounds__(256) void embedding_join(
       for (int w = 0; w < 256 / WAVE; ++w) found += ends[w];
       later += found;
       __syncthreads();
-      if (found < JOIN_LOOKS * 256) break;
+      if (found < (unsigned)looks * 256) break;
     }
     const size_t j = (size_t)(q % strips) * COLS + l * CW;
     double s[CW];
 #pragma unroll
     for (int i = 0; i < CW; ++i) s[i] = 0.0;
     if (j < n) { /* CW > 1: n is a multiple of it */
-      for (size_t k0 = slice; k0 <= later; k0 += JOIN_ROWS * JOIN_SLICES) {
-        P t[JOIN_ROWS][CW];
+      auto add = [&]<int R>() { /* R partial rows on their way */
+        for (size_t k0 = slice; k0 <= later; k0 += R * JOIN_SLICES) {
+          P t[R][CW];
 #pragma unroll
-        for (int u = 0; u < JOIN_ROWS; ++u) {
-          const size_t k = k0 + u * JOIN_SLICES <= later ? k0 + u * JOIN_SLICES : k0;
-          load_pack_nt<P, CW>(partials + ((c + k) * 2 + (k == 0 ? 1 : 0)) * n + j, t[u]);
+          for (int u = 0; u < R; ++u) {
+            const size_t k = k0 + u * JOIN_SLICES <= later ? k0 + u * JOIN_SLICES : k0;
+            load_pack_nt<P, CW>(partials + ((c + k) * 2 + (k == 0 ? 1 : 0)) * n + j, t[u]);
+          }
+#pragma unroll
+          for (int u = 0; u < R; ++u)
+#pragma unroll
+            for (int i = 0; i < CW; ++i) s[i] += k0 + u * JOIN_SLICES <= later ? (double)t[u][i] : 0.0;
         }
-#pragma unroll
-        for (int u = 0; u < JOIN_ROWS; ++u)
-#pragma unroll
-          for (int i = 0; i < CW; ++i) s[i] += k0 + u * JOIN_SLICES <= later ? (double)t[u][i] : 0.0;
-      }
+      };
+      if (later < JOIN_SLICES) add.template operator()<1>();
+      else if (later < 4 * JOIN_SLICES) add.template operator()<4>();
+      else add.template operator()<8>();
     }
 #pragma unroll
     for (int i = 0; i < CW; ++i) part[slice][l * CW + i] = s[i];

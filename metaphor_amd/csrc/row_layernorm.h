@@ -881,7 +881,8 @@ inline void layernorm_reverse_as(const NormPlan& plan, const T* x, const T* gain
         else { if (loose) as.template operator()<false, true>(); else as.template operator()<false, false>(); }
       };
       /* the next rows' loads in flight where the registers hold them (r32 [8192, 4096] 70.6 us against 73.4
-       * without; r16 at two packs a lane spills and loses by it, 45.9 against 42.7) */
+       * without; r16 at two packs a lane takes 153 registers then, one workgroup a unit instead of two: [16384, 2048]
+       * 46.5 against 41.1) */
       if (plan.sub == 8) go.template operator()<8, 1, false, 512>();
       else if (plan.sub == 16) go.template operator()<16, 1, false, 512>();
       else if (plan.sub == 32) go.template operator()<32, 1, false, 512>();
