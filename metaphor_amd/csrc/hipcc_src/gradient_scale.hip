@@ -3,8 +3,10 @@
 // clipped_k = grads_k * min(1, max_norm / norm[0]) for `count` tensors, with the norm that an earlier
 // gradient_norm left on the device (tensors of several types: one gradient_norm each, alpha = 1 from the
 // second on, then one gradient_scale each). grads, clipped and sizes are host arrays as in
-// gradient_norm; clipped_k may be grads_k, and a norm of at most max_norm then writes nothing. A norm
-// that is infinite or NaN gives zeros and NaNs as the formula does: the caller sees it in norm.
+// gradient_norm; clipped_k may be grads_k, and a norm of at most max_norm then writes nothing. A result
+// that overlaps another result or another gradient is refused: what it holds would depend on which
+// workgroup comes first. A norm that is infinite or NaN gives zeros and NaNs as the formula does: the
+// caller sees it in norm.
 extern "C" void launch_gradient_scale_Scalar(
   const void* grads,
   const void* clipped,
