@@ -158,6 +158,11 @@ static __global__ __launch_bounds__(NORM_THREADS) void gradient_norm_finish(cons
   }
 }
 
+/* The smallest normal number of P. A factor below it has lost bits, or all of them, where g * max_norm / norm
+ * still is a number of P (r32 gradients of 1e38 and a largest norm of 1e-6): such a product is taken as
+ * (g / norm) * max_norm in fp64, whose first factor is at most one and whose second is given. */
+template <class P> __device__ constexpr double norm_least_factor() { return sizeof(P) == 4 ? 0x1p-126 : 0x1p-1022; }
+
 /* FUSED: norm_in is what the squares left, `partials` sums; the first workgroup writes the norm. */
 template <class T, bool FUSED, bool APART>
 __global__ __launch_bounds__(NORM_THREADS) void gradient_scaled(NormTable<T, APART> t, const double* norm_in, unsigned partials, double* norm_out, double max_norm) {
@@ -167,6 +172,7 @@ __global__ __launch_bounds__(NORM_THREADS) void gradient_scaled(NormTable<T, APA
   const NormPiece<T> piece(t, blockIdx.x);
   const T* src = t.src[piece.run] + piece.lo;
   T* dst = APART ? t.dst[piece.run] + piece.lo : const_cast<T*>(src);
+  double inverse = 0.0; /* 1 / norm where the factor has left P's normal range, else zero */
   /* what to scale by; false: nothing to do in place */
   auto factor_of = [&](P& factor) {
     double total;
@@ -178,7 +184,10 @@ __global__ __launch_bounds__(NORM_THREADS) void gradient_scaled(NormTable<T, APA
       total = norm_in[0];
     }
     const bool within = total <= max_norm;
-    factor = within ? (P)1 : (P)(max_norm / total);
+    const double ratio = within ? 1.0 : max_norm / total;
+    factor = (P)ratio;
+    if constexpr (sizeof(T) != 2) /* an r16 result is zero there either way */
+      if (ratio < norm_least_factor<P>()) inverse = 1.0 / total;
     return !(within && src == dst);
   };
   typename vec_of<T, W>::type v[NORM_PACKS];
@@ -186,10 +195,14 @@ __global__ __launch_bounds__(NORM_THREADS) void gradient_scaled(NormTable<T, APA
   auto scaled = [&](int u, P (&out)[W]) {
 #pragma unroll
     for (int j = 0; j < W; ++j) out[j] = (P)v[u][j] * factor;
+    if (sizeof(T) == 2 || inverse == 0.0) return;
+#pragma unroll
+    for (int j = 0; j < W; ++j) out[j] = (P)((double)v[u][j] * inverse * max_norm);
   };
   if (piece.whole()) { /* on its own from load to store: 203 M elements 262 us, 267 where both share the loops */
 #pragma unroll
     for (int u = 0; u < NORM_PACKS; ++u) v[u] = __builtin_nontemporal_load(reinterpret_cast<const VL*>(src + piece.at(u)));
+    asm volatile("" ::: "memory"); /* on their way while the norm is read, not behind it (261 us, 266 without) */
     if (!factor_of(factor)) return;
 #pragma unroll
     for (int u = 0; u < NORM_PACKS; ++u) {

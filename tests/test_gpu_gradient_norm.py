@@ -238,3 +238,37 @@ def test_a_tensor_of_more_than_2_32_elements():
     assert torch.equal(t[where], torch.full((5,), 2.0, dtype=F16, device="cuda")) and bool((small == 1.0).all())
     t[where] = 0
     assert not bool(t.any())
+
+
+@pytest.mark.parametrize("dtype,value,limits", [(F32, 1e38, (1.0, 1e-2, 1e-6, 1e-30)), (F32, 3e38, (1e-8,)), (F64, 1e150, (1e-150, 1e-200)),
+                                                (F16, 6e4, (1e-30, 1e-40))])
+@pytest.mark.parametrize("count", [1, 9, 5003, 9000001])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_factors_below_the_range_of_the_type(dtype, value, limits, count, in_place):
+    """max_norm / norm is subnormal or zero in the computing type (for r64 in fp64 too), g * max_norm / norm is not:
+    g / norm is at most one, so it is computed from that here. Both ways of scaling, up to 2048 pieces and more."""
+    for limit in limits:
+        g = normal((count,), dtype, 3, 0.25 * value)
+        g = torch.where(g.abs() > value, torch.full_like(g, value), g)
+        src, norm = g.cuda(), a_norm()
+        out = src if in_place else torch.full_like(src, float("nan"))
+        G.say(f"clip {dtype} {count} values of {value} to {limit}")
+        clip([src], [out], dtype, norm, limit)
+        ref, bound = P.gradient_norm([g])
+        P.close(norm, np.array([ref]), np.array([bound]), f"norm of {value}")
+        want = P.host64(g) / ref * limit
+        # the norm is off by 1e-12 of itself, the product is rounded a few times in fp64, the result once
+        P.close(out, want, (4 * P.U[F64] + P.HALF[dtype] + 1e-12) * np.abs(want) + P.TINY[dtype], f"clipped {value} to {limit}")
+
+
+def test_a_largest_norm_of_zero_and_an_infinite_norm():
+    """A factor of zero: zeros with their sign kept out of the comparison, NaN where the gradient is infinite."""
+    for dtype in TYPES:
+        t = normal((3000,), dtype, 1)
+        out, norm = torch.full_like(t, float("nan")).cuda(), a_norm()
+        clip([t.cuda()], [out], dtype, norm, 0.0)
+        assert not bool(out.any()) and float(norm) > 0
+        t[17] = float("inf")
+        src = t.cuda()
+        clip([src], [src], dtype, norm, 0.5)
+        assert float(norm) == float("inf") and bool(torch.isnan(src[17])) and int((src != 0).sum()) == 1
