@@ -53,12 +53,13 @@ __device__ __forceinline__ typename vec_of<T, W>::type whole_pack(const RowPacks
 template <class T, int W, int G, bool LOOSE>
 __global__ __launch_bounds__(256) void embedding_rows(
     const T* table, const void* tokens, T* y, typename precision<T>::type scale, unsigned wide, unsigned v, size_t m,
-    size_t n, unsigned strips) {
+    size_t n, unsigned strips, unsigned first_block) {
   using P = typename precision<T>::type;
   const int sub = threadIdx.x / G, lane = threadIdx.x % G;
   const RowPacks<T, W, LOOSE> rp(n);
-  const size_t row = (size_t)(blockIdx.x / strips) * (256 / G) + sub;
-  const int p = (int)(blockIdx.x % strips) * G + lane;
+  const unsigned block = first_block + blockIdx.x;
+  const size_t row = (size_t)(block / strips) * (256 / G) + sub;
+  const int p = (int)(block % strips) * G + lane;
   if (row >= m || p >= rp.npk) return;
   const unsigned k = token_key(tokens, wide != 0, row, v);
   P out[W];
@@ -372,14 +373,15 @@ template <class T, int W, int G, bool BLEND, bool LOOSE>
 __global__ __launch_bounds__(256) void embedding_sum(
     const unsigned* keys, const unsigned* places, const T* dy, T* grads, typename precision<T>::type* partials,
     unsigned* crossing, unsigned* list, typename precision<T>::type scale, typename precision<T>::type alpha, unsigned v, size_t m, size_t n,
-    size_t chunk, unsigned strips, unsigned sum_blocks, size_t row_begin, unsigned fill_rows) {
+    size_t chunk, unsigned strips, unsigned sum_blocks, size_t row_begin, unsigned fill_rows, unsigned first_block) {
   using P = typename precision<T>::type;
   using V = typename vec_of<T, W>::type;
   const RowPacks<T, W, LOOSE> rp(n);
+  const unsigned block = first_block + blockIdx.x;
 
-  if (blockIdx.x >= sum_blocks) {
+  if (block >= sum_blocks) {
     __shared__ unsigned named[FILL_MOST];
-    const size_t row0 = row_begin + (size_t)(blockIdx.x - sum_blocks) * fill_rows;
+    const size_t row0 = row_begin + (size_t)(block - sum_blocks) * fill_rows;
     const unsigned rows = (unsigned)(v - row0 < fill_rows ? v - row0 : fill_rows);
     if (threadIdx.x < rows) {
       const unsigned key = (unsigned)row0 + threadIdx.x;
@@ -393,12 +395,12 @@ __global__ __launch_bounds__(256) void embedding_sum(
 
   constexpr int U = 8; /* rows on their way at once */
   const int sub = threadIdx.x / G, lane = threadIdx.x % G;
-  const size_t c = (size_t)(blockIdx.x / strips) * (256 / G) + sub;
-  const int p = (int)(blockIdx.x % strips) * G + lane;
+  const size_t c = (size_t)(block / strips) * (256 / G) + sub;
+  const int p = (int)(block % strips) * G + lane;
   size_t lo = c * chunk, hi = lo + chunk < m ? lo + chunk : m;
   bool begun = false, goes_on = false; /* the first id began in another chunk, the last one goes on in another */
   constexpr int NG = G < WAVE ? WAVE / G : 1; /* chunks a wavefront */
-  const size_t first = G < WAVE ? (size_t)blockIdx.x / strips * (256 / G) + threadIdx.x / WAVE * NG : c;
+  const size_t first = G < WAVE ? (size_t)(block / strips) * (256 / G) + threadIdx.x / WAVE * NG : c;
   unsigned at_edge[NG + 1];
 #pragma unroll
   for (int g = 0; g <= NG; ++g) at_edge[g] = edge_key(keys, m, (first + g) * chunk, (unsigned)chunk);
@@ -481,16 +483,17 @@ constexpr int DIRECT_WORDS = DIRECT_MOST / WAVE;
 template <class T, int W, int G, bool BLEND, bool LOOSE>
 __global__ __launch_bounds__(256) void embedding_direct(
     const void* tokens, unsigned wide, const T* dy, T* grads, typename precision<T>::type scale, typename precision<T>::type alpha, unsigned v, unsigned m,
-    size_t n, unsigned strips, unsigned place_blocks, unsigned fill_rows) {
+    size_t n, unsigned strips, unsigned place_blocks, unsigned fill_rows, unsigned first_block) {
   using P = typename precision<T>::type;
   using V = typename vec_of<T, W>::type;
   const RowPacks<T, W, LOOSE> rp(n);
   __shared__ unsigned keys[DIRECT_MOST];
+  const unsigned block = first_block + blockIdx.x;
   const unsigned mine = threadIdx.x < m ? token_key(tokens, wide != 0, threadIdx.x, v) : v;
 
-  if (blockIdx.x >= place_blocks) {
+  if (block >= place_blocks) {
     __shared__ unsigned named[FILL_MOST];
-    const size_t row0 = (size_t)(blockIdx.x - place_blocks) * fill_rows;
+    const size_t row0 = (size_t)(block - place_blocks) * fill_rows;
     const unsigned rows = (unsigned)(v - row0 < fill_rows ? v - row0 : fill_rows);
     if (threadIdx.x < rows) named[threadIdx.x] = 0;
     __syncthreads();
@@ -502,8 +505,8 @@ __global__ __launch_bounds__(256) void embedding_direct(
   keys[threadIdx.x] = mine;
   __syncthreads();
   const int sub = threadIdx.x / G, lane = threadIdx.x % G;
-  const unsigned i = (blockIdx.x / strips) * (256 / G) + sub;
-  const int p = (int)(blockIdx.x % strips) * G + lane;
+  const unsigned i = (block / strips) * (256 / G) + sub;
+  const int p = (int)(block % strips) * G + lane;
   const unsigned key = i < m ? keys[i] : v;
   /* the places of this group's id, a bit each, by votes of the whole wavefront for each of its groups */
   unsigned long long places[DIRECT_WORDS];
@@ -689,14 +692,27 @@ template <class T> inline EmbeddingScratch embedding_scratch(size_t m, size_t n)
   return s;
 }
 
-/* Lanes for a strip of a row's packs: the next power of two up to 256. */
+/* Lanes for a strip of a row's packs: the next power of two, from 8 to 256. */
+inline size_t strip_lanes(size_t packs) {
+  size_t lanes = 8;
+  while (lanes < 256 && lanes < packs) lanes *= 2;
+  return lanes;
+}
 template <class F> inline void for_strip(size_t packs, F&& f) {
-  if (packs <= 8) f.template operator()<8>();
-  else if (packs <= 16) f.template operator()<16>();
-  else if (packs <= 32) f.template operator()<32>();
-  else if (packs <= 64) f.template operator()<64>();
-  else if (packs <= 128) f.template operator()<128>();
-  else f.template operator()<256>();
+  switch (strip_lanes(packs)) {
+    case 8: f.template operator()<8>(); break;
+    case 16: f.template operator()<16>(); break;
+    case 32: f.template operator()<32>(); break;
+    case 64: f.template operator()<64>(); break;
+    case 128: f.template operator()<128>(); break;
+    default: f.template operator()<256>();
+  }
+}
+/* Workgroups of 256 threads that take `rows` rows of `packs` packs: a strip of 256 / lanes rows each. */
+struct StripGrid { size_t strips, blocks; };
+inline StripGrid strip_grid(size_t rows, size_t packs) {
+  const size_t lanes = strip_lanes(packs), strips = (packs + lanes - 1) / lanes, each = 256 / lanes;
+  return {strips, (rows + each - 1) / each * strips};
 }
 
 inline void embedding_check(const void* tokens, size_t id_bytes, size_t v, size_t m, size_t n) {
@@ -716,14 +732,18 @@ inline void embedding_forward(const T* table, const void* tokens, T* y, double s
   if (m == 0 || n == 0) return;
   const bool loose = !(aligned16(table) && aligned16(y) && n % W == 0);
   const size_t packs = (n + W - 1) / W;
+  const StripGrid rows = strip_grid(m, packs);
+  require(rows.blocks < 0x7fffffffull, "embedding: too many rows for one call");
   for_strip(packs, [&]<int G>() {
-    const size_t strips = (packs + G - 1) / G, blocks = (m + 256 / G - 1) / (256 / G) * strips;
-    require(blocks < 0x7fffffffull, "embedding: too many rows for one grid");
-    const dim3 grid((unsigned)blocks), block(256);
-    if (loose) embedding_rows<T, W, G, true><<<grid, block, 0, stream>>>(table, tokens, y, (P)scale, id_bytes == 8, (unsigned)v, m, n, (unsigned)strips);
-    else embedding_rows<T, W, G, false><<<grid, block, 0, stream>>>(table, tokens, y, (P)scale, id_bytes == 8, (unsigned)v, m, n, (unsigned)strips);
+    in_launches(rows.blocks, [&](dim3 grid, unsigned first) {
+      auto go = [&]<bool LOOSE>() {
+        embedding_rows<T, W, G, LOOSE><<<grid, dim3(256), 0, stream>>>(table, tokens, y, (P)scale, id_bytes == 8, (unsigned)v, m, n, (unsigned)rows.strips, first);
+      };
+      if (loose) go.template operator()<true>();
+      else go.template operator()<false>();
+      MP_CHECK_LAUNCH();
+    });
   });
-  MP_CHECK_LAUNCH();
 }
 
 template <class T>
@@ -738,23 +758,32 @@ inline void embedding_reverse(const void* tokens, const T* dy, T* grads, void* s
   const bool loose = !(aligned16(dy) && aligned16(grads) && n % W == 0);
   const size_t packs = (n + W - 1) / W;
   const unsigned wide = id_bytes == 8, fill_rows = embedding_fill_rows(n * sizeof(T));
+  const size_t fill_all = alpha == 1.0 ? 0 : (v + fill_rows - 1) / fill_rows; /* workgroups for all rows of the table */
   if (m <= DIRECT_MOST) {
-    const size_t fill = alpha == 1.0 ? 0 : (v + fill_rows - 1) / fill_rows;
+    const StripGrid places = strip_grid(m, packs);
+    require(places.blocks + fill_all < 0x7fffffffull, "embedding reverse: too many rows for one call");
     for_strip(packs, [&]<int G>() {
-      const size_t strips = (packs + G - 1) / G, places = (m + 256 / G - 1) / (256 / G) * strips;
-      require(places + fill < 0x7fffffffull, "embedding reverse: too many rows for one grid");
-      if (places + fill == 0) return; /* no token, and nothing to clear or to scale */
-      const dim3 grid((unsigned)(places + fill)), block(256);
-      auto go = [&]<bool BLEND, bool LOOSE>() {
-        embedding_direct<T, W, G, BLEND, LOOSE><<<grid, block, 0, stream>>>(tokens, wide, dy, grads, (P)scale, (P)alpha, (unsigned)v, (unsigned)m, n,
-                                                                            (unsigned)strips, (unsigned)places, fill_rows);
-      };
-      if (alpha != 0.0) { if (loose) go.template operator()<true, true>(); else go.template operator()<true, false>(); }
-      else { if (loose) go.template operator()<false, true>(); else go.template operator()<false, false>(); }
+      in_launches(places.blocks + fill_all, [&](dim3 grid, unsigned first) { /* none: no token, and nothing to clear or to scale */
+        auto go = [&]<bool BLEND, bool LOOSE>() {
+          embedding_direct<T, W, G, BLEND, LOOSE><<<grid, dim3(256), 0, stream>>>(tokens, wide, dy, grads, (P)scale, (P)alpha, (unsigned)v, (unsigned)m, n,
+                                                                                  (unsigned)places.strips, (unsigned)places.blocks, fill_rows, first);
+        };
+        if (alpha != 0.0) { if (loose) go.template operator()<true, true>(); else go.template operator()<true, false>(); }
+        else { if (loose) go.template operator()<false, true>(); else go.template operator()<false, false>(); }
+        MP_CHECK_LAUNCH();
+      });
     });
-    MP_CHECK_LAUNCH();
     return;
   }
+  /* every grid, before the first launch */
+  const size_t chunk = embedding_chunk(m, n * sizeof(T)), chunks = (m + chunk - 1) / chunk;
+  const StripGrid sums = strip_grid(chunks, packs);
+  require(sums.blocks + fill_all < 0x7fffffffull, "embedding reverse: too many rows for one call");
+  constexpr bool FP32 = sizeof(P) == 4;
+  const bool four = FP32 && n % 4 == 0; /* columns a thread of the join: four where the partial rows are 16-byte aligned */
+  const size_t join_cols = JOIN_LANES * (four ? 4 : 1), join_strips = (n + join_cols - 1) / join_cols, joins = (chunks - 1) * join_strips;
+  require(chunks * join_strips < 0x7fffffffull, "embedding reverse: too many rows for one call");
+
   const EmbeddingScratch at = embedding_scratch<T>(m, n);
   char* base = static_cast<char*>(scratch);
   auto words = [&](size_t offset) { return reinterpret_cast<unsigned*>(base + offset); };
@@ -803,30 +832,25 @@ inline void embedding_reverse(const void* tokens, const T* dy, T* grads, void* s
     sorted_places = places[(passes - 1) & 1];
   }
 
-  const size_t chunk = embedding_chunk(m, n * sizeof(T)), chunks = (m + chunk - 1) / chunk;
   const size_t row_begin = cleared / n; /* rows from here on are still to be looked at, the first of them perhaps half cleared */
   const size_t fill = alpha == 1.0 ? 0 : (v - row_begin + fill_rows - 1) / fill_rows;
   for_strip(packs, [&]<int G>() {
-    const size_t strips = (packs + G - 1) / G, sums = (chunks + 256 / G - 1) / (256 / G) * strips;
-    require(sums + fill < 0x7fffffffull, "embedding reverse: too many rows for one grid");
-    const dim3 grid((unsigned)(sums + fill)), block(256);
-    auto go = [&]<bool BLEND, bool LOOSE>() {
-      embedding_sum<T, W, G, BLEND, LOOSE><<<grid, block, 0, stream>>>(sorted_keys, sorted_places, dy, grads, partials, crossing, list, (P)scale, (P)alpha,
-                                                                       (unsigned)v, m, n, chunk, (unsigned)strips, (unsigned)sums, row_begin, fill_rows);
-    };
-    if (alpha != 0.0) { if (loose) go.template operator()<true, true>(); else go.template operator()<true, false>(); }
-    else { if (loose) go.template operator()<false, true>(); else go.template operator()<false, false>(); }
+    in_launches(sums.blocks + fill, [&](dim3 grid, unsigned first) {
+      auto go = [&]<bool BLEND, bool LOOSE>() {
+        embedding_sum<T, W, G, BLEND, LOOSE><<<grid, dim3(256), 0, stream>>>(sorted_keys, sorted_places, dy, grads, partials, crossing, list, (P)scale, (P)alpha,
+                                                                             (unsigned)v, m, n, chunk, (unsigned)sums.strips, (unsigned)sums.blocks, row_begin,
+                                                                             fill_rows, first);
+      };
+      if (alpha != 0.0) { if (loose) go.template operator()<true, true>(); else go.template operator()<true, false>(); }
+      else { if (loose) go.template operator()<false, true>(); else go.template operator()<false, false>(); }
+      MP_CHECK_LAUNCH();
+    });
   });
-  MP_CHECK_LAUNCH();
   if (chunks > 1) {
-    /* four columns a thread where the partial rows are 16-byte aligned */
-    constexpr bool FP32 = sizeof(P) == 4;
-    const bool four = FP32 && n % 4 == 0;
-    const size_t cols = JOIN_LANES * (four ? 4 : 1), strips = (n + cols - 1) / cols, cap = (size_t)compute_units() * 8;
-    require(chunks * strips < 0x7fffffffull, "embedding reverse: too many rows for one grid");
-    const dim3 grid((unsigned)((chunks - 1) * strips < cap ? (chunks - 1) * strips : cap)), block(256);
+    const size_t cap = (size_t)compute_units() * 8;
+    const dim3 grid((unsigned)(joins < cap ? joins : cap)), block(256);
     auto go = [&]<int CW, bool BLEND>() {
-      embedding_join<T, CW, BLEND><<<grid, block, 0, stream>>>(sorted_keys, partials, crossing, list, grads, (P)scale, (P)alpha, m, n, chunk, (unsigned)strips);
+      embedding_join<T, CW, BLEND><<<grid, block, 0, stream>>>(sorted_keys, partials, crossing, list, grads, (P)scale, (P)alpha, m, n, chunk, (unsigned)join_strips);
     };
     if (four) { if constexpr (FP32) { if (alpha != 0.0) go.template operator()<4, true>(); else go.template operator()<4, false>(); } }
     else { if (alpha != 0.0) go.template operator()<1, true>(); else go.template operator()<1, false>(); }

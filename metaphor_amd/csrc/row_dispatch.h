@@ -305,6 +305,15 @@ inline unsigned row_grid(size_t m, int G) {
   return (unsigned)blocks;
 }
 
+/* A launch has fewer than 2^32 threads; beyond, the runtime launches what is left of the number in 32 bits and
+ * reports nothing. `blocks` workgroups (fewer than 2^31) of up to 256 threads in as many launches as that takes,
+ * each kernel told the number of its first one: f(grid, first). */
+constexpr size_t LAUNCH_BLOCKS = (size_t)1 << 23;
+template <class F> inline void in_launches(size_t blocks, F&& f) {
+  for (size_t first = 0; first < blocks; first += LAUNCH_BLOCKS)
+    f(dim3((unsigned)(blocks - first < LAUNCH_BLOCKS ? blocks - first : LAUNCH_BLOCKS)), (unsigned)first);
+}
+
 }  // namespace mp
 
 #endif

@@ -258,3 +258,40 @@ def test_many_tokens_and_rows_beyond_32_bit_offsets(m):
     assert torch.equal(g[tokens[live]], dy[live] * 0.5)
     g[tokens[live]] = 0
     assert not bool(g.any())
+
+
+@pytest.mark.parametrize("m,n", [(2 ** 29 + 3, 1), (2 ** 23 + 10, 2056)])
+def test_more_rows_than_a_launch_has_threads(m, n):
+    """A launch takes fewer than 2^32 threads: 2^24 workgroups of 32 narrow rows, or of half a row."""
+    v = 211
+    table = normal((v, n), F16, 1).cuda()
+    tokens = (torch.arange(m, dtype=torch.int32, device="cuda") * 7) % (v + 1) - 1  # -1: a padded place
+    y = torch.full((m, n), float("nan"), dtype=F16, device="cuda")
+    G.say(f"lookup of {m} rows of {n}")
+    lookup(table, tokens, y, 1.0)
+    torch.cuda.synchronize()
+    rows = torch.cat([torch.zeros(1, n, dtype=F16, device="cuda"), table])
+    step = max(1, 2 ** 28 // n)
+    for lo in range(0, m, step):
+        assert torch.equal(y[lo:lo + step], rows[(tokens[lo:lo + step] + 1).long()]), f"rows from {lo}"
+
+
+@pytest.mark.parametrize("m", [1, 256, 300, 9000])
+@pytest.mark.parametrize("alpha", [0.0, 0.5])
+def test_more_rows_to_clear_than_a_launch_has_threads(m, alpha):
+    """A table of 2^30 + 64 narrow rows, which takes 2^24 + 1 workgroups to clear or to scale; by every way of
+    ordering the places, named rows at both ends."""
+    v = 2 ** 30 + 64
+    g = torch.full((v, 1), 4.0, dtype=F16, device="cuda")
+    tokens = torch.cat([torch.arange(m // 2), torch.arange(v - (m - m // 2), v)])[torch.randperm(m, generator=gen(4))]
+    dy = normal((m, 1), F16, 2).cuda()
+    sc = scratch_for(F16, v, m, 1)
+    G.say(f"lookup reverse of {m} tokens, a table of {v} rows, alpha {alpha}")
+    lookup_reverse(tokens.cuda(), dy, g, sc.t, 0.5, alpha)
+    torch.cuda.synchronize()
+    sc.check("scratch")
+    named, rest = tokens.cuda(), 4.0 * alpha
+    want = (dy.float() * 0.5 + rest).to(F16)  # every id once: exact in fp32, then rounded once
+    assert torch.equal(g[named], want)
+    g[named] = rest
+    assert bool((g == rest).all())

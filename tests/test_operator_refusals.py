@@ -69,3 +69,18 @@ def test_workspace_sizes():
         for count in (1, 96, 97, 1000):
             assert kernels.mpGradientNormScratchBytes(key, count) % 8 == 0 and kernels.mpGradientNormScratchBytes(key, count) >= 8
         assert kernels.mpGradientNormScratchBytes(key, 0) == 0
+
+
+MANY = [
+    # every refusal comes before the first launch, which without a GPU ends the process with another message
+    ("embedding_i_ij", f"{FAKE}, {FAKE}, {FAKE}, 1.0, 8, 10, (1 << 31) - 1, 1 << 20", "too many rows"),
+    ("embedding_i_ij_reverse", f"{FAKE}, {FAKE}, {FAKE}, {FAKE}, 1.0, 0.0, 8, (1 << 32) - 2, 9000, 1 << 20", "too many rows"),
+    ("embedding_i_ij_reverse", f"{FAKE}, {FAKE}, {FAKE}, {FAKE}, 1.0, 0.0, 8, (1 << 32) - 2, 300, 1 << 20", "too many rows"),
+    ("embedding_i_ij_reverse", f"{FAKE}, {FAKE}, {FAKE}, {FAKE}, 1.0, 0.0, 8, (1 << 32) - 2, 20, 1 << 20", "too many rows"),
+    ("embedding_i_ij_reverse", f"{FAKE}, {FAKE}, {FAKE}, {FAKE}, 1.0, 1.0, 8, 10, (1 << 31) - 1, 1 << 30", "too many rows"),
+]
+
+
+@pytest.mark.parametrize("stem,args,message", MANY)
+def test_more_than_a_launch_takes_is_refused_before_the_first_one(stem, args, message):
+    test_a_call_that_cannot_be_right_is_refused(stem, args, message)
