@@ -712,13 +712,13 @@ __global__ __launch_bounds__(BLOCK) void layernorm_rev_rows(
 constexpr int NORM_FINISH_LANES = 8, NORM_FINISH_SLICES = 32;
 template <class T>
 __global__ __launch_bounds__(NORM_FINISH_LANES * NORM_FINISH_SLICES) void layernorm_grads_finish(
-    const typename precision<T>::type* partials, T* dg, T* db, double alpha, int rows, size_t n) {
+    const typename precision<T>::type* partials, T* dg, T* db, double alpha, int rows, size_t n, unsigned first_block) {
   using P = typename precision<T>::type;
   constexpr int CW = PACK_BYTES / (int)sizeof(P), COLS = NORM_FINISH_LANES * CW;
   __shared__ double part[NORM_FINISH_SLICES][COLS + 1];
   const int c = threadIdx.x % NORM_FINISH_LANES, slice = threadIdx.x / NORM_FINISH_LANES;
   const size_t apart = partial_apart<T>(n), width = 2 * apart;
-  const size_t col = ((size_t)blockIdx.x * NORM_FINISH_LANES + c) * CW;
+  const size_t block = first_block + blockIdx.x, col = (block * NORM_FINISH_LANES + c) * CW;
   double s[CW];
 #pragma unroll
   for (int i = 0; i < CW; ++i) s[i] = 0.0;
@@ -740,7 +740,7 @@ __global__ __launch_bounds__(NORM_FINISH_LANES * NORM_FINISH_SLICES) void layern
 #pragma unroll
   for (int i = 0; i < CW; ++i) part[slice][c * CW + i] = s[i];
   __syncthreads();
-  const size_t at = (size_t)blockIdx.x * COLS + threadIdx.x, j = at < apart ? at : at - apart;
+  const size_t at = block * COLS + threadIdx.x, j = at < apart ? at : at - apart;
   if (threadIdx.x < COLS && at < width && j < n) {
     T* out = at < apart ? dg : db;
     if (!out) return;
@@ -900,9 +900,10 @@ inline void layernorm_reverse_as(const NormPlan& plan, const T* x, const T* gain
   }
   if ((!dg && !db) || (m > 0 && plan.nv != 0 && rows == 1)) return;
   constexpr size_t cols = NORM_FINISH_LANES * PACK_BYTES / sizeof(P);
-  const dim3 grid((unsigned)((2 * partial_apart<T>(n) + cols - 1) / cols)), block(NORM_FINISH_LANES * NORM_FINISH_SLICES);
-  layernorm_grads_finish<T><<<grid, block, 0, stream>>>(partials, dg, db, alpha, (int)rows, n);
-  MP_CHECK_LAUNCH();
+  in_launches((2 * partial_apart<T>(n) + cols - 1) / cols, [&](dim3 grid, unsigned first) {
+    layernorm_grads_finish<T><<<grid, dim3(NORM_FINISH_LANES * NORM_FINISH_SLICES), 0, stream>>>(partials, dg, db, alpha, (int)rows, n, first);
+    MP_CHECK_LAUNCH();
+  });
 }
 
 template <class T>

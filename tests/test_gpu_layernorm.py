@@ -316,3 +316,27 @@ def test_many_rows_in_place(dtype, m, n, alpha):
     refs, bounds = P.layernorm_reverse(x, gain, dy, EPS, dtype, alpha, old)
     for name, got, ref, bound in zip(("dx", "dg", "db"), (X, dg, db), refs, bounds):
         P.close(got.t, ref, bound, f"layernorm {name} {what}")
+
+
+@pytest.mark.parametrize("dtype,n", [(F32, 2 ** 28), (F64, 2 ** 27)])
+def test_vectors_of_more_columns_than_a_launch_has_threads(dtype, n):
+    """The last sums of dg and db by more workgroups than fewer than 2^32 threads make. Values whose sums are exact: x
+    +1, -1, ... and dy +1, +1, -1, -1, ..., so every mean is zero, h is x * r and dx is dy * r."""
+    x = torch.ones(2, n, dtype=dtype, device="cuda")
+    x[:, 1::2] = -1.0
+    dy = torch.ones(2, n, dtype=dtype, device="cuda")
+    dy[:, 2::4] = -1.0
+    dy[:, 3::4] = -1.0
+    dy[1] *= 2.0
+    dx, dg, db = torch.full_like(x, float("nan")), torch.full_like(x[0], float("nan")), torch.full_like(x[0], float("nan"))
+    sc = scratch_for(dtype, 2, n)
+    G.say(f"layernorm reverse {dtype} of rows of {n}")
+    reverse(x, None, dy, dx, dg, db, sc.t, eps=1.0)
+    torch.cuda.synchronize()
+    sc.check("scratch")
+    r = 2.0 ** -0.5
+    # a reciprocal square root good to one ulp and four roundings
+    near = lambda got, ref: float((got - ref).abs().max()) <= 8 * P.U[dtype] * 3.0  # noqa: E731
+    assert torch.equal(db, dy[0] + dy[1])
+    assert near(dg, (dy[0] + dy[1]) * x[0] * r)
+    assert near(dx, dy * r)
