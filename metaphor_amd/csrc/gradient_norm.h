@@ -306,7 +306,8 @@ inline void gradient_check(const void* grads, const void* outs, const void* size
     require(!outs || static_cast<const void* const*>(outs)[k] != nullptr, "gradient clip: a result's address is NULL");
     require(size < 0x1000000000000ull, "gradient norm: a tensor's size is out of range");
     pieces += (size * sizeof(T) + NORM_PIECE - 1) / NORM_PIECE;
-    require(pieces < 0x7fffffffull, "gradient norm: too many elements");
+    /* the scaling's workgroups take a piece each, and a launch has fewer than 2^32 threads: 256 GiB of tensors */
+    require(pieces < (outs ? ((size_t)1 << 32) / NORM_THREADS : 0x7fffffffull), "gradient norm: too many elements");
   }
 }
 

@@ -72,6 +72,10 @@ def test_workspace_sizes():
 
 
 MANY = [
+    # 2^24 workgroups of 256 threads are 2^32 threads, more than a launch takes
+    ("gradient_scale", f"A({FAKE}), A({FAKE}), L(1 << 36), {FAKE}, 1.0, 1", "too many elements"),
+    ("gradient_scale", f"A({FAKE}, {FAKE + (1 << 44)}), A({FAKE}, {FAKE + (1 << 44)}), L(1 << 35, 1 << 35), {FAKE}, 1.0, 2", "too many elements"),
+    ("gradient_clip", f"A({FAKE}), A({FAKE + (1 << 44)}), L(1 << 36), {FAKE}, {FAKE}, 1.0, 1", "too many elements"),
     # every refusal comes before the first launch, which without a GPU ends the process with another message
     ("embedding_i_ij", f"{FAKE}, {FAKE}, {FAKE}, 1.0, 8, 10, (1 << 31) - 1, 1 << 20", "too many rows"),
     ("embedding_i_ij_reverse", f"{FAKE}, {FAKE}, {FAKE}, {FAKE}, 1.0, 0.0, 8, (1 << 32) - 2, 9000, 1 << 20", "too many rows"),
