@@ -318,6 +318,30 @@ def test_many_rows_in_place(dtype, m, n, alpha):
         P.close(got.t, ref, bound, f"layernorm {name} {what}")
 
 
+@pytest.mark.parametrize("n", [8, 100, 1024, 4096, 5121, 8192, 12288, 16384, 40960])
+def test_half_precision_rows_far_from_zero(n):
+    """A mean a thousand times the spread, in the type whose pivot is the mean of all elements: sums about it come from
+    sum - held * pivot. At 1000 an r16 step is 0.5, which the rows hold as their spread."""
+    for mean in (1000.0, -30.0):
+        x, gain, bias, dy = normal((5, n), F16, 1, 1.0, mean), normal((n,), F16, 2, 0.2, 1.0), normal((n,), F16, 3), normal((5, n), F16, 4)
+        check_forward(x, gain, bias, f"r16 n={n} mean {mean}")
+        check_reverse(x, gain, dy, f"r16 n={n} mean {mean}")
+
+
+@pytest.mark.parametrize("n", [8, 100, 1024, 4096, 5121, 16384, 40960])
+def test_subnormal_half_precision_values(n):
+    """dy and x below the normal range of r16, of one sign, so that their sums and their means count: rows of little
+    spread scale them up by up to 1 / sqrt(eps)."""
+    for m in (1, 5, 300):
+        dy = (normal((m, n), F16, 4).abs().double() * 1e-6).to(F16)
+        assert bool((dy > 0).any()) and float(dy.max()) < 2.0 ** -14
+        gain = normal((n,), F16, 2, 0.2, 1.0)
+        check_reverse(normal((m, n), F16, 1, 2.0, 0.5), gain, dy, f"r16 [{m},{n}] subnormal dy")
+        x = (normal((m, n), F16, 1).abs().double() * 1e-6).to(F16)
+        check_forward(x, gain, None, f"r16 [{m},{n}] subnormal x", eps=1e-14)
+        check_reverse(x, gain, dy, f"r16 [{m},{n}] subnormal x and dy", eps=1e-9)
+
+
 @pytest.mark.parametrize("dtype,n", [(F32, 2 ** 28), (F64, 2 ** 27)])
 def test_vectors_of_more_columns_than_a_launch_has_threads(dtype, n):
     """The last sums of dg and db by more workgroups than fewer than 2^32 threads make. Values whose sums are exact: x
