@@ -260,6 +260,29 @@ def test_many_tokens_and_rows_beyond_32_bit_offsets(m):
     assert not bool(g.any())
 
 
+@pytest.mark.parametrize("m", [200, 256, 300, 9000])
+def test_a_common_id_keeps_small_addends(m):
+    """One id whose first row is 1 and the others a little under half a step of 1 (in the type it is added in): a sum that
+    goes through all places in turn in that type loses every one of them, m - 1 times 2^-24. The sums' bound is that of at
+    most 64 additions in the type."""
+    v, n = 5, 20
+    for dtype in (F32, F64):
+        tokens = torch.full((m,), 3)
+        dy = torch.full((m, n), 0.99 * P.U[dtype], dtype=dtype)
+        dy[0] = 1.0
+        dt, sc = torch.full((v, n), float("nan"), dtype=dtype, device="cuda"), scratch_for(dtype, v, m, n)
+        G.say(f"lookup reverse {dtype} of a common id, {m} places")
+        lookup_reverse(tokens.cuda(), dy.cuda(), dt, sc.t, 1.0)
+        torch.cuda.synchronize()
+        # 0.99 * (m - 1) / 2^53 beside 1 is more than fp64 sums hold exactly: long double
+        ref = np.zeros((v, n), np.longdouble)
+        ref[3] = np.longdouble(1.0) + (m - 1) * np.longdouble(float(dy[1, 0]))
+        err = np.abs(P.host64(dt).astype(np.longdouble) - ref)
+        bound = (64 + 4 + 1) * P.U[dtype] * np.abs(ref)
+        print(f"[bound] {dtype} {m} places: worst err/bound={float((err[3] / bound[3]).max()):.3f}", flush=True)
+        assert bool((err <= bound).all()), float((err[3] / bound[3]).max())
+
+
 @pytest.mark.parametrize("m,n", [(2 ** 29 + 3, 1), (2 ** 23 + 10, 2056)])
 def test_more_rows_than_a_launch_has_threads(m, n):
     """A launch takes fewer than 2^32 threads: 2^24 workgroups of 32 narrow rows, or of half a row."""
