@@ -23,6 +23,11 @@ fn last_size(t: Tensor) usize {
     return s[s.len - 1];
 }
 
+// an index counts within its class (src/core/graph.zig:34-41)
+fn same(a: Tensor, b: Tensor) bool {
+    return a.ptr == b.ptr and a.idx == b.idx and a.class == b.class;
+}
+
 pub fn forward(x: Tensor, gain: Tensor, bias: Tensor, eps: f64) Tensor {
     return forward_impl(x.ptr, x, gain, bias, eps);
 }
@@ -33,8 +38,10 @@ pub fn forward_impl(graph: *Graph, x: Tensor, gain: Tensor, bias: Tensor, eps: f
     std.debug.assert(gain.dtype() == x.dtype());
     std.debug.assert(bias.len() == n);
     std.debug.assert(bias.dtype() == x.dtype());
-    // one gradient vector cannot take both sums
-    std.debug.assert(bias.idx != gain.idx);
+    // one launch writes the three gradients
+    std.debug.assert(!same(x, gain));
+    std.debug.assert(!same(x, bias));
+    std.debug.assert(!same(gain, bias));
     const m = if (n == 0) 0 else x.len() / n;
 
     const out = graph.tensor(.{ .class = .hid, .dtype = x.dtype(), .sizes = x.sizes() });
