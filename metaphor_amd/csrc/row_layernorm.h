@@ -849,6 +849,16 @@ inline void layernorm_forward(const T* x, const T* gain, const T* bias, T* y, do
   layernorm_forward_as<T>(layernorm_forward_plan<T>((n + W - 1) / W), x, gain, bias, y, eps, m, n, stream);
 }
 
+/* A few rows: one workgroup takes them all in two turns or up to four, and one launch of two is saved, as long as
+ * there is little to read: it walks alone what several would take at once. One against two launches, us:
+ *   two turns     r32 [2,8192] 6.1, 7.7   r64 [2,4096] 7.8, 8.2   r16 [2,16384] 8.1, 9.4   beyond 64 KiB: r32
+ *                 [2,12288] 9.6, 9.7   [2,16384] 12.7, 11.8   r64 [2,8192] 19.6, 16.9
+ *   three, four   r16 [3,8192] 6.7, 7.7   r64 [3,2048] 6.7, 7.5   r32 [3,4096] 5.7, 7.6   beyond 48 KiB: r32 [4,4096]
+ *                 6.7, 7.5   r16 [16,2048] 9.2, 8.2   r64 [4,2048] 8.1, 7.5   r32 [4,16384] 22.8, 11.9 */
+inline bool layernorm_one_workgroup(size_t workgroups, size_t bytes) {
+  return workgroups <= 2 ? bytes <= 65536 : workgroups <= 4 && bytes <= 49152;
+}
+
 template <class T>
 inline void layernorm_reverse_as(const NormPlan& plan, const T* x, const T* gain, const T* dy, T* dx, T* dg, T* db, void* scratch, double eps, double alpha,
                                  size_t m, size_t n, hipStream_t stream) {
@@ -868,9 +878,7 @@ inline void layernorm_reverse_as(const NormPlan& plan, const T* x, const T* gain
       else { if (loose) go.template operator()<false, true>(); else go.template operator()<false, false>(); }
     } else {
       rows = norm_grid(plan, m);
-      /* a few rows: one workgroup takes them all in up to four turns, and one launch is saved (r32 [16, 512] 4.7
-       * us against 7.1, [64, 256] 6.3 against 7.2, [4, 4096] 6.7 against 7.2) */
-      if (rows <= 4) rows = 1;
+      if (layernorm_one_workgroup(rows, m * n * sizeof(T))) rows = 1;
       require(rows <= layernorm_partial_rows(m), "layernorm reverse: more partial rows than the workspace holds");
       const dim3 grid((unsigned)rows), block(norm_block(plan));
       auto go = [&]<int SUB, int NV, bool PAIR, int BLOCK>() {

@@ -364,3 +364,26 @@ def test_vectors_of_more_columns_than_a_launch_has_threads(dtype, n):
     assert torch.equal(db, dy[0] + dy[1])
     assert near(dg, (dy[0] + dy[1]) * x[0] * r)
     assert near(dx, dy * r)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,kib", [(1, 0), (2, 64), (3, 48), (4, 48)])
+def test_what_one_workgroup_takes(dtype, m, kib):
+    """Two rows of 64 KiB together, three or four of 48, are left to one workgroup, which writes dg and db itself and
+    leaves the workspace alone; more go to a workgroup each, which leave their sums there. Rows long enough for a
+    workgroup to hold one at a time, a little below and a little above."""
+    each = kib * 1024 // dtype.itemsize // m // 16 * 16 - 16
+    for n, alone in (((16384 // dtype.itemsize, True),) if m == 1 else ((each, True), (each + 32, False), (32768 // dtype.itemsize, m * 32 <= kib))):
+        x, dy, gain = normal((m, n), dtype, 1), normal((m, n), dtype, 2), normal((n,), dtype, 3)
+        dx, dg, db, sc = guarded(x), guarded(gain), guarded(gain), scratch_for(dtype, m, n)
+        sc.t.fill_(255)
+        what = f"{dtype} [{m},{n}] by {'one workgroup' if alone else 'several'}"
+        G.say(f"layernorm reverse {what}")
+        reverse(x.cuda(), gain.cuda(), dy.cuda(), dx.t, dg.t, db.t, sc.t)
+        torch.cuda.synchronize()
+        for k in (dx, dg, db, sc):
+            k.check(what)
+        assert bool((sc.t == 255).all()) == alone, what
+        refs, bounds = P.layernorm_reverse(x, gain, dy, EPS, dtype)
+        for name, got, ref, bound in zip(("dx", "dg", "db"), (dx, dg, db), refs, bounds):
+            P.close(got.t, ref, bound, f"layernorm {name} {what}")
