@@ -796,14 +796,16 @@ template <class T> inline NormPlan layernorm_forward_plan(size_t packs) {
   if (gw > NORM_WAVES) return {WAVE, 0, 0, 0, 0};
   return {WAVE, nv, gw, 1, waves / gw ? waves / gw : 1};
 }
-template <class T> inline NormPlan layernorm_reverse_plan(size_t packs) {
+/* plain: nothing is blended, and rows are whole packs on aligned addresses */
+template <class T> inline NormPlan layernorm_reverse_plan(size_t packs, bool plain) {
   if (packs <= 8) return {8, 1, 1, 64, 2};
   if (packs <= 16) return {16, 1, 1, 32, 2};
   if (packs <= 32) return {32, 1, 1, 16, 2};
   if (packs <= 64) return {WAVE, 1, 1, 16, 1};
   /* r16 rows of more than 24 KiB: four packs a lane and no more than eight wavefronts, which leaves room for the
-   * next row ([2048, 16384] 55.6 -> 52.5 us) */
-  const int nv = packs <= (sizeof(T) == 2 ? 1536 : 2048) ? 2 : 4, gw = norm_waves(packs, nv), rows = gw < 8 ? 8 / gw : 1;
+   * next row ([3051, 16384] 68.6 us, two packs on sixteen wavefronts 72.0; 300 rows 28.0 and 25.1), but not for what
+   * a blend reads too (114 us against 86) or a cut pack takes ([3051, 16383] 96.8 against 87.3) */
+  const int nv = packs <= (sizeof(T) == 2 && plain ? 1536 : 2048) ? 2 : 4, gw = norm_waves(packs, nv), rows = gw < 8 ? 8 / gw : 1;
   if (gw > NORM_WAVES) return {WAVE, 0, 0, 0, 0};
   return {WAVE, nv, gw, rows, sizeof(T) == 2 && nv == 2 && gw > 1 && gw <= 8 ? 2 : 1};
 }
@@ -859,6 +861,10 @@ inline bool layernorm_one_workgroup(size_t workgroups, size_t bytes) {
   return workgroups <= 2 ? bytes <= 65536 : workgroups <= 4 && bytes <= 49152;
 }
 
+template <class T> inline bool layernorm_reverse_loose(const T* x, const T* gain, const T* dy, const T* dx, size_t n) {
+  return !(aligned16(x) && aligned16(dy) && aligned16(dx) && (!gain || aligned16(gain)) && n % (PACK_BYTES / sizeof(T)) == 0);
+}
+
 template <class T>
 inline void layernorm_reverse_as(const NormPlan& plan, const T* x, const T* gain, const T* dy, T* dx, T* dg, T* db, void* scratch, double eps, double alpha,
                                  size_t m, size_t n, hipStream_t stream) {
@@ -867,7 +873,7 @@ inline void layernorm_reverse_as(const NormPlan& plan, const T* x, const T* gain
   P* partials = static_cast<P*>(scratch);
   size_t rows = 0;
   if (m > 0) {
-    const bool loose = !(aligned16(x) && aligned16(dy) && aligned16(dx) && (!gain || aligned16(gain)) && n % W == 0);
+    const bool loose = layernorm_reverse_loose(x, gain, dy, dx, n);
     if (plan.nv == 0) {
       rows = layernorm_partial_rows(m);
       const dim3 grid((unsigned)rows), block(STREAM_THREADS);
@@ -923,7 +929,8 @@ inline void layernorm_reverse(const T* x, const T* gain, const T* dy, T* dx, T* 
   require(dg != db || dg == nullptr, "layernorm reverse: gain_grads and bias_grads must be different vectors");
   require(m == 0 || scratch != nullptr, "layernorm reverse: scratch must hold mpLayernormReverseScratchBytes bytes");
   require(reinterpret_cast<uintptr_t>(scratch) % 16 == 0, "layernorm reverse: scratch must be aligned to its sums in packs (16-byte aligned)");
-  layernorm_reverse_as<T>(layernorm_reverse_plan<T>((n + W - 1) / W), x, gain, dy, dx, dg, db, scratch, eps, alpha, m, n, stream);
+  const bool plain = alpha == 0.0 && !layernorm_reverse_loose(x, gain, dy, dx, n);
+  layernorm_reverse_as<T>(layernorm_reverse_plan<T>((n + W - 1) / W, plain), x, gain, dy, dx, dg, db, scratch, eps, alpha, m, n, stream);
 }
 
 }  // namespace mp

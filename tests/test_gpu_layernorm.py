@@ -387,3 +387,12 @@ def test_what_one_workgroup_takes(dtype, m, kib):
         refs, bounds = P.layernorm_reverse(x, gain, dy, EPS, dtype)
         for name, got, ref, bound in zip(("dx", "dg", "db"), (dx, dg, db), refs, bounds):
             P.close(got.t, ref, bound, f"layernorm {name} {what}")
+
+
+@pytest.mark.parametrize("n", [12280, 12288, 12289, 12296, 14001, 16376, 16384, 16385])
+@pytest.mark.parametrize("alpha", [0.0, 1.0])
+def test_half_precision_rows_around_the_plans_of_long_rows(n, alpha):
+    """Where two packs a lane become four, which differs with a blend; more rows than workgroups, whole and ragged."""
+    x, gain, dy = normal((600, n), F16, n, 2.0, 0.5), normal((n,), F16, 2, 0.2, 1.0), normal((600, n), F16, 4)
+    check_reverse(x, gain, dy, f"r16 [600,{n}] alpha {alpha}", alpha=alpha)
+    check_reverse(x[:7], gain, dy[:7], f"r16 [7,{n}] alpha {alpha} off alignment", shifts=(1, 1, 0, 1, 1), alpha=alpha)
