@@ -513,6 +513,36 @@ static int launch_cost(int launches) {
   return 0;
 }
 
+/* Reverses that enqueue more or fewer kernels by their sizes count as one launch, whatever they are. */
+static int launch_counts(mp::Stream stream) {
+  mp::Graph* G = mp::Graph::init({stream, mp::Mode::train});
+  Rng r{31};
+  for (const size_t m : {(size_t)3, (size_t)700}) {
+    const size_t n = 64, v = 20;
+    const auto hx = r.normal(m * n, 0, 1), hg = r.normal(n, 1, 0.1), hb = r.normal(n, 0, 0.1), ht = r.normal(v * n, 0, 1);
+    mp::Tensor x = leaf(G, mp::TensorClass::wgt, {m, n}, hx), g = leaf(G, mp::TensorClass::wgt, {n}, hg), b = leaf(G, mp::TensorClass::wgt, {n}, hb);
+    mp::Tensor h = mp::ops::layernorm(x, g, b, 1e-5);
+    set_grad(h, hx);
+    size_t l = G->launches;
+    h.reverse(mp::ReverseCleanup::keep);
+    CHECK(G->launches == l + 1);
+    std::vector<int32_t> ids(m);
+    for (size_t i = 0; i < m; ++i) ids[i] = (int32_t)(i % v);
+    void* device_ids = mpMemAlloc(m * sizeof(int32_t), stream->context);
+    mpMemcpyHtoD(device_ids, ids.data(), m * sizeof(int32_t), stream->context);
+    mpStreamSynchronize(stream->context);
+    mp::Tensor table = leaf(G, mp::TensorClass::wgt, {v, n}, ht), y = mp::ops::embedding(table, {device_ids, m, sizeof(int32_t)});
+    set_grad(y, hx);
+    l = G->launches;
+    y.reverse(mp::ReverseCleanup::keep);
+    CHECK(G->launches == l + 1);
+    mpStreamSynchronize(stream->context);
+    mpMemFree(device_ids, stream->context);
+  }
+  G->deinit();
+  return 0;
+}
+
 int main(int argc, char** argv) {
   if (argc == 3 && std::string(argv[1]) == "--launch-cost") return launch_cost(atoi(argv[2]) > 0 ? atoi(argv[2]) : 2000);
   if (argc != 2) {
@@ -535,6 +565,7 @@ int main(int argc, char** argv) {
   printf("host_check: softmax / rmsnorm through the graph ok\n");
   if (token_model(stream)) return 1;
   printf("host_check: embedding / layer norm / clipping through the graph ok\n");
+  if (launch_counts(stream)) return 1;
   if (matrix_ops(stream)) return 1;
   printf("host_check: inner products, permutate, reduce / broadcast, checkpoint files ok\n");
 

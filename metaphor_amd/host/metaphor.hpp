@@ -216,7 +216,8 @@ class Graph {
    * that changes from call to call is an argument of the same kernel) */
   std::vector<std::string> runtime_chains_;
 
-  /* kernels enqueued through this graph so far (fusion is observable through it) */
+  /* kernels enqueued through this graph so far (fusion is observable through it); a launcher that goes by the sizes for
+   * how many kernels it enqueues (the reverses of layernorm and embedding, clip_gradients' calls) counts as one */
   size_t launches = 0;
 
   /* materialise every pending node; called before anything mutates tensor bytes in place */
