@@ -774,8 +774,12 @@ template <class T> inline size_t layernorm_reverse_scratch_bytes(size_t m, size_
  *   as many workgroups a unit as make 12 wavefronts of four-byte rows (r32 [4099, 5120] 29.9 us at ten, 30.6 at
  *   twenty) and 20 of two-byte ones (r16 [8192, 2560] 16.6 at 18, 17.9 at 12, 18.5 at 30), whose lanes hold
  *   half the bytes;
- *   rows of more than 64 KiB, r16 rows of more than 32 KiB, read three times: what is left of the registers
- *   spills (forward r32 [1024, 32768] 78 us against 87, r16 39 against 59). */
+ *   forward rows of more than 64 KiB, r16 rows of more than 32 KiB, read three times: what is left of the registers
+ *   spills (r32 [1024, 32768] 78 us against 87, r16 39 against 59).
+ * The reverse holds twice the operands and the sums of the columns, and spills in rows of more than 32 KiB (r32 12 registers
+ * of a lane, 21 ragged, r64 37 to 55; r16 of more than 32 KiB 149 to 205), but reading a row's operands five times
+ * and the sums from memory costs more for as long as a workgroup can hold the row, 64 KiB in every type: r32 [2034,
+ * 12288] 71 us against 199, r64 [1525, 8192] 93 against 173, r16 [2500, 20000] 224 against 624. */
 struct NormPlan {
   int sub, nv, gw, rows, per_cu;
 };
@@ -906,8 +910,12 @@ inline void layernorm_reverse_as(const NormPlan& plan, const T* x, const T* gain
         else if (block.x <= 512) go.template operator()<WAVE, 2, false, 512>();
         else go.template operator()<WAVE, 2, false, 1024>();
       } else {
-        if constexpr (sizeof(T) == 2) { if (block.x <= 512) go.template operator()<WAVE, 4, true, 512>(); else go.template operator()<WAVE, 4, false, 1024>(); }
-        else go.template operator()<WAVE, 4, false, 1024>();
+        if constexpr (sizeof(T) == 2) {
+          if (block.x <= 512) { /* the plan's plain rows */
+            require(alpha == 0.0 && !loose, "layernorm reverse: a plan for plain rows");
+            layernorm_rev_rows<T, W, WAVE, 4, false, false, true, 512><<<grid, block, 0, stream>>>(x, gain, dy, dx, dg, db, partials, (P)eps, (P)alpha, m, n, plan.gw);
+          } else go.template operator()<WAVE, 4, false, 1024>();
+        } else go.template operator()<WAVE, 4, false, 1024>();
       }
     }
     MP_CHECK_LAUNCH();
