@@ -780,8 +780,8 @@ EXTERN_C void launch_gradient_norm_r64(
 /* second on, then one gradient_scale each). grads, clipped and sizes are host arrays as in */
 /* gradient_norm; clipped_k may be grads_k, and a norm of at most max_norm then writes nothing. A result */
 /* that overlaps another result or another gradient is refused: what it holds would depend on which */
-/* workgroup comes first; so are 256 GiB of tensors or more in one call. A norm that is infinite or NaN gives zeros and NaNs as the formula does: the */
-/* caller sees it in norm. */
+/* workgroup comes first. 256 GiB of tensors or more in one call are refused too. A norm that is infinite */
+/* or NaN gives zeros and NaNs as the formula does: the caller sees it in norm. */
 EXTERN_C void launch_gradient_scale_r16(
   const void* grads,
   const void* clipped,
